@@ -59,7 +59,7 @@ class CandleB200Error(RuntimeError):
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
-            f"{LIB_PATH} is missing: build the CUDA extension first (python -m candle_b200.build); "
+            f"{LIB_PATH} is missing: build the CUDA extension first (python candle_b200/build.py); "
             "there is no CPU fallback"
         )
     lib = ctypes.CDLL(LIB_PATH)

@@ -28,7 +28,7 @@ E_TIMEOUT = -6
 
 def _load() -> ctypes.CDLL:
     if not os.path.exists(NCCL_LIB_PATH):
-        raise ImportError(f"{NCCL_LIB_PATH} is missing: build it first (python -m candle_b200.build)")
+        raise ImportError(f"{NCCL_LIB_PATH} is missing: build it first (python candle_b200/build.py)")
     import torch  # noqa: F401  (brings torch's libnccl.so.2 into the process before ours asks for it)
 
     lib = ctypes.CDLL(NCCL_LIB_PATH)
