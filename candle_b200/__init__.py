@@ -13,12 +13,17 @@ from .ops import (
     FLAG_FORCE_GENERIC,
     FLAG_FORCE_LANEROW,
     FLAG_FORCE_REPLAY,
+    embedding_backward,
     embedding_rms_norm,
+    embedding_scaled,
     index_select,
     layer_norm,
     layer_norm_slow,
     qembedding_rms_norm,
+    qk_norm_rope,
+    qk_norm_rope_backward,
     rms_norm,
+    rms_norm_backward,
     rms_norm_rows,
     rms_norm_slow,
     rope,
@@ -32,6 +37,7 @@ from .quantized import GgmlDType, QTensor
 
 __all__ = [
     "CandleError", "InvalidIndex", "rms_norm", "layer_norm", "rms_norm_slow", "layer_norm_slow", "rms_norm_rows", "softmax_last_dim", "rope", "rope_i", "rope_thd", "index_select", "embedding_rms_norm",
+    "embedding_scaled", "embedding_backward", "rms_norm_backward", "qk_norm_rope", "qk_norm_rope_backward",
     "qembedding_rms_norm", "PinnedNormPipeline", "Embedding", "LayerNorm", "RmsNorm", "QEmbedding", "QTensor", "GgmlDType",
     "FLAG_FAST_SUM", "FLAG_FORCE_LANEROW", "FLAG_FORCE_GENERIC", "FLAG_FORCE_REPLAY",
 ]

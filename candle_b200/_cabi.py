@@ -37,6 +37,16 @@ SIGNATURES = {
     "cb200_qembedding_rms_norm_row_owner": [
         _vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i32, _i64, _f32, _int, _int, _i64, _i64, _int, _vp, _vp,
     ],
+    "cb200_embedding_scaled": [_vp, _vp, _vp, _i64, _i32, _i64, _f32, _int, _int, _vp, _vp],
+    "cb200_embedding_backward": [
+        _vp, _i64, _vp, _vp, _i64, _i32, _i64, _f32, _i64, _int, _int, _int, _int, _vp, _i64, _vp, _vp,
+    ],
+    "cb200_embedding_backward_workspace": [_i64, _i32, _i64, _vp],
+    "cb200_rms_norm_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _int, _vp, _i64, _vp],
+    "cb200_rms_norm_backward_workspace": [_i64, _i32, _vp],
+    "cb200_qk_norm_rope": [_vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "cb200_qk_norm_rope_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
+    "cb200_qk_norm_rope_backward_workspace": [_i32, _vp],
 }
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2

@@ -3,6 +3,7 @@
 // beyond a thread-local error message.
 #include <cstdarg>
 #include <cstdio>
+#include <utility>
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -129,6 +130,79 @@ int check_lookup(const char* name, const void* table, const void* ids, const voi
   if (vocab < 0 || hidden < 0 || n_ids < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape", name);
   if (n_ids > 0 && hidden > 0 && (table == nullptr || ids == nullptr || out == nullptr))
     return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  return CB200_OK;
+}
+
+int check_workspace(const char* name, const void* workspace, int64_t given, int64_t needed) {
+  if (given < needed || (needed > 0 && workspace == nullptr))
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: the workspace has %lld bytes, %lld are needed", name, (long long)given,
+                (long long)needed);
+  if (!aligned16(workspace)) return fail(CB200_E_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", name);
+  return CB200_OK;
+}
+
+int check_table_grad_shape(const char* name, int64_t vocab, int32_t hidden, int64_t n_ids) {
+  if (vocab < 0 || hidden < 0 || n_ids < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape", name);
+  if (vocab >= (int64_t(1) << 31) || n_ids >= (int64_t(1) << 31))
+    return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: the rows of the table and the ids must be fewer than 2^31", name);
+  return CB200_OK;
+}
+
+int check_rms_backward_shape(const char* name, int64_t rows, int32_t cols) {
+  if (rows < 0 || cols < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape [%lld, %d]", name, (long long)rows, cols);
+  if (cols == 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: rows of zero columns cannot be normalised", name);
+  if (rows > (int64_t(1) << 40)) return fail(CB200_E_INVALID_ARGUMENT, "%s: too many rows", name);
+  return CB200_OK;
+}
+
+int check_qk(const char* name, const cb200_qk_args* a) {
+  if (a == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null arguments", name);
+  if (!valid_dtype(a->dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", name, a->dtype);
+  if (a->table_dtype != a->dtype && a->table_dtype != CB200_DTYPE_F32)
+    return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: the dtype code of cos / sin is %d (expected the heads' or F32)", name, a->table_dtype);
+  if (a->positions != nullptr && !valid_id_dtype(a->position_dtype))
+    return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported positions dtype code %d", name, a->position_dtype);
+  if (a->batch < 0 || a->tokens < 0 || a->max_positions < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape", name);
+  if (a->batch > (int64_t(1) << 31) || a->tokens > (int64_t(1) << 31) || a->batch * a->tokens > (int64_t(1) << 31))
+    return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: more than 2^31 tokens", name);
+  if (a->dim <= 0 || a->rotary <= 0 || a->rotary > a->dim || a->rotary % 2 != 0)
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: %d rotated columns of %d (expected an even number of at most the head size)", name,
+                a->rotary, a->dim);
+  if (a->positions == nullptr && a->tokens > a->max_positions)
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: %lld tokens, but cos / sin have %lld positions", name, (long long)a->tokens,
+                (long long)a->max_positions);
+  if (a->q_weight == nullptr || a->k_weight == nullptr || (a->max_positions > 0 && (a->cos == nullptr || a->sin == nullptr)))
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  return CB200_OK;
+}
+
+// `like`: the input whose heads `h` has to match; outputs may not map two elements to one address.
+int check_heads(const char* name, const cb200_heads* h, const cb200_heads* like, const cb200_qk_args* a, bool written) {
+  if (h == nullptr || like == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null arguments", name);
+  if (h->heads < 0 || h->heads != like->heads)
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: %d heads where %d are expected", name, h->heads, like->heads);
+  if (h->heads == 0 || a->batch == 0 || a->tokens == 0) return CB200_OK;
+  if (h->data == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  if (h->batch_stride < 0 || h->token_stride < 0 || h->head_stride < 0)
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: negative stride", name);
+  if (!written) return CB200_OK;
+  // dimensions by stride: each must step over everything inside it
+  int64_t dims[3][2] = {{h->batch_stride, a->batch}, {h->token_stride, a->tokens}, {h->head_stride, h->heads}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (dims[j][0] > dims[j + 1][0]) {
+        std::swap(dims[j][0], dims[j + 1][0]);
+        std::swap(dims[j][1], dims[j + 1][1]);
+      }
+  int64_t extent = a->dim;
+  bool overlap = false;
+  for (const auto& d : dims) {
+    if (d[1] <= 1) continue;
+    overlap |= d[0] < extent;
+    extent += d[0] * (d[1] - 1);
+  }
+  if (overlap)
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: the output's rows overlap", name);
   return CB200_OK;
 }
 
@@ -574,6 +648,154 @@ int cb200_qembedding_route_rows(const void* qtable, int qtype, const void* ids, 
   const int row_bytes = hidden / cb200::qblock_elems(qtype) * cb200::qblock_bytes(qtype);
   return cuda_result(cb200::launch_qroute_rows(static_cast<const unsigned char*>(qtable), ids, id_dtype, vocab, vocab_begin,
                                                vocab_end, status, n_ids, row_bytes, dsts, n_dsts, row_bounds, stream),
+                     name);
+}
+
+int cb200_embedding_scaled(const void* table, const void* ids, void* out, int64_t vocab, int32_t hidden, int64_t n_ids,
+                           float scale, int dtype, int id_dtype, cb200_status* status, cb200_stream_t stream) {
+  const TraceRange trace("cb200_embedding_scaled");
+  const char* name = "cb200_embedding_scaled";
+  if (!valid_dtype(dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", name, dtype);
+  const int rc = check_lookup(name, table, ids, out, vocab, hidden, n_ids, id_dtype);
+  if (rc != CB200_OK) return rc;
+  cb200::ScaledLookupArgs a{};
+  a.table = table;
+  a.ids = ids;
+  a.out = out;
+  a.vocab = vocab;
+  a.n_ids = n_ids;
+  a.hidden = hidden;
+  a.scale = scale;
+  a.id_dtype = id_dtype;
+  a.status = status;
+  return cuda_result(cb200::launch_embedding_scaled(dtype, a, stream), name);
+}
+
+int cb200_embedding_backward_workspace(int64_t vocab, int32_t hidden, int64_t n_ids, int64_t* bytes) {
+  const char* name = "cb200_embedding_backward_workspace";
+  const int rc = check_table_grad_shape(name, vocab, hidden, n_ids);
+  if (rc != CB200_OK) return rc;
+  if (bytes == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null pointer", name);
+  *bytes = cb200::table_grad_workspace(vocab, hidden, n_ids);
+  return CB200_OK;
+}
+
+int cb200_embedding_backward(const void* grad, int64_t grad_stride, const void* ids, void* out, int64_t vocab,
+                             int32_t hidden, int64_t n_ids, float scale, int64_t padding_id, int accumulate, int dtype,
+                             int out_dtype, int id_dtype, void* workspace, int64_t workspace_bytes, cb200_status* status,
+                             cb200_stream_t stream) {
+  const TraceRange trace("cb200_embedding_backward");
+  const char* name = "cb200_embedding_backward";
+  if (!valid_dtype(dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", name, dtype);
+  if (out_dtype != dtype && out_dtype != CB200_DTYPE_F32)
+    return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: the output's dtype code is %d (expected the gradient's or F32)", name, out_dtype);
+  int rc = check_table_grad_shape(name, vocab, hidden, n_ids);
+  if (rc != CB200_OK) return rc;
+  if (!valid_id_dtype(id_dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported ids dtype code %d", name, id_dtype);
+  if (grad_stride < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative row stride", name);
+  if (hidden > 0 && ((n_ids > 0 && (grad == nullptr || ids == nullptr)) || (vocab > 0 && out == nullptr)))
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  if (n_ids > 0 && hidden > 0) {
+    rc = check_workspace(name, workspace, workspace_bytes, cb200::table_grad_workspace(vocab, hidden, n_ids));
+    if (rc != CB200_OK) return rc;
+  }
+  cb200::TableGradArgs a{};
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  a.ids = ids;
+  a.out = out;
+  a.vocab = vocab;
+  a.n_ids = n_ids;
+  a.padding_id = padding_id;
+  a.hidden = hidden;
+  a.scale = scale;
+  a.id_dtype = id_dtype;
+  a.accumulate = accumulate ? 1 : 0;
+  a.status = status;
+  return cuda_result(cb200::launch_table_grad(dtype, out_dtype, a, workspace, stream), name);
+}
+
+int cb200_rms_norm_backward_workspace(int64_t rows, int32_t cols, int64_t* bytes) {
+  const char* name = "cb200_rms_norm_backward_workspace";
+  const int rc = check_rms_backward_shape(name, rows, cols);
+  if (rc != CB200_OK) return rc;
+  if (bytes == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null pointer", name);
+  *bytes = cb200::rms_backward_workspace(rows, cols);
+  return CB200_OK;
+}
+
+int cb200_rms_norm_backward(const void* grad, const void* x, const void* alpha, const void* grad_sum, void* dx, void* dalpha,
+                            int64_t rows, int32_t cols, float eps, int dtype, void* workspace, int64_t workspace_bytes,
+                            cb200_stream_t stream) {
+  const TraceRange trace("cb200_rms_norm_backward");
+  const char* name = "cb200_rms_norm_backward";
+  if (!valid_dtype(dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", name, dtype);
+  int rc = check_rms_backward_shape(name, rows, cols);
+  if (rc != CB200_OK) return rc;
+  if (dalpha == nullptr || (rows > 0 && (grad == nullptr || x == nullptr || alpha == nullptr || dx == nullptr)))
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  if (rows > 0) {
+    rc = check_workspace(name, workspace, workspace_bytes, cb200::rms_backward_workspace(rows, cols));
+    if (rc != CB200_OK) return rc;
+  }
+  cb200::RmsBackwardArgs a{};
+  a.grad = grad;
+  a.x = x;
+  a.alpha = alpha;
+  a.grad_sum = grad_sum;
+  a.dx = dx;
+  a.dalpha = static_cast<float*>(dalpha);
+  a.rows = rows;
+  a.n = cols;
+  a.eps = eps;
+  return cuda_result(cb200::launch_rms_backward(dtype, a, workspace, stream), name);
+}
+
+int cb200_qk_norm_rope(const cb200_heads* q, const cb200_heads* k, const cb200_heads* q_out, const cb200_heads* k_out,
+                       const cb200_qk_args* args, cb200_status* status, cb200_stream_t stream) {
+  const TraceRange trace("cb200_qk_norm_rope");
+  const char* name = "cb200_qk_norm_rope";
+  int rc = check_qk(name, args);
+  if (rc != CB200_OK) return rc;
+  const cb200_heads* in[2] = {q, k};
+  const cb200_heads* out[2] = {q_out, k_out};
+  for (int i = 0; i < 2; ++i) {
+    rc = check_heads(name, in[i], in[i], args, false);
+    if (rc == CB200_OK) rc = check_heads(name, out[i], in[i], args, true);
+    if (rc != CB200_OK) return rc;
+  }
+  return cuda_result(cb200::launch_qk_norm_rope(*q, *k, *q_out, *k_out, *args, status, stream), name);
+}
+
+int cb200_qk_norm_rope_backward_workspace(int32_t dim, int64_t* bytes) {
+  const char* name = "cb200_qk_norm_rope_backward_workspace";
+  if (dim < 0 || bytes == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: bad argument", name);
+  *bytes = cb200::qk_backward_workspace(dim);
+  return CB200_OK;
+}
+
+int cb200_qk_norm_rope_backward(const cb200_heads* grad_q, const cb200_heads* grad_k, const cb200_heads* q,
+                                const cb200_heads* k, const cb200_heads* dq, const cb200_heads* dk, void* dq_weight,
+                                void* dk_weight, const cb200_qk_args* args, void* workspace, int64_t workspace_bytes,
+                                cb200_status* status, cb200_stream_t stream) {
+  const TraceRange trace("cb200_qk_norm_rope_backward");
+  const char* name = "cb200_qk_norm_rope_backward";
+  int rc = check_qk(name, args);
+  if (rc != CB200_OK) return rc;
+  const cb200_heads* x[2] = {q, k};
+  const cb200_heads* g[2] = {grad_q, grad_k};
+  const cb200_heads* d[2] = {dq, dk};
+  for (int i = 0; i < 2; ++i) {
+    rc = check_heads(name, x[i], x[i], args, false);
+    if (rc == CB200_OK) rc = check_heads(name, g[i], x[i], args, false);
+    if (rc == CB200_OK) rc = check_heads(name, d[i], x[i], args, true);
+    if (rc != CB200_OK) return rc;
+  }
+  if (dq_weight == nullptr || dk_weight == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  rc = check_workspace(name, workspace, workspace_bytes, cb200::qk_backward_workspace(args->dim));
+  if (rc != CB200_OK) return rc;
+  return cuda_result(cb200::launch_qk_norm_rope_backward(*grad_q, *grad_k, *q, *k, *dq, *dk, static_cast<float*>(dq_weight),
+                                                         static_cast<float*>(dk_weight), *args, workspace, status, stream),
                      name);
 }
 

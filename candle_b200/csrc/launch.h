@@ -109,4 +109,59 @@ cudaError_t launch_qroute_rows(const unsigned char* qtable, const void* ids, int
 cudaError_t launch_dequantize_flat(int qtype, int out_dtype, const void* blocks, void* out, int64_t n_vec,
                                    cudaStream_t stream);  // n_vec: groups of 8 elements
 
+// Scaled lookup and the table's gradient (embedding_train.cu)
+struct ScaledLookupArgs {
+  const void* table;  // [vocab, hidden]
+  const void* ids;
+  void* out;          // [n_ids, hidden]
+  int64_t vocab, n_ids;
+  int hidden;
+  float scale;
+  int id_dtype;
+  cb200_status* status;
+};
+cudaError_t launch_embedding_scaled(int dtype, const ScaledLookupArgs& a, cudaStream_t stream);
+
+struct TableGradArgs {
+  const void* grad;  // [n_ids, hidden], rows grad_stride elements apart
+  int64_t grad_stride;
+  const void* ids;
+  void* out;  // [vocab, hidden]
+  int64_t vocab, n_ids, padding_id;
+  int hidden;
+  float scale;
+  int id_dtype;
+  int accumulate;
+  cb200_status* status;
+};
+int64_t table_grad_workspace(int64_t vocab, int hidden, int64_t n_ids);
+cudaError_t launch_table_grad(int dtype, int out_dtype, const TableGradArgs& a, void* workspace, cudaStream_t stream);
+
+// Gradient of the RMS norm (rms_backward.cu)
+struct RmsBackwardArgs {
+  const void* grad;
+  const void* x;
+  const void* alpha;
+  const void* grad_sum;  // optional
+  void* dx;
+  float* dalpha;
+  int64_t rows;
+  int n;
+  float eps;
+};
+int64_t rms_backward_workspace(int64_t rows, int n);
+cudaError_t launch_rms_backward(int dtype, const RmsBackwardArgs& a, void* workspace, cudaStream_t stream);
+// out[c] = sum over p of partials[p * cols + c], in the order of p within fixed groups (rms_backward.cu)
+cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, cudaStream_t stream);
+
+// Head norms with the rotation in the same pass (head_norm.cu)
+cudaError_t launch_qk_norm_rope(const cb200_heads& q, const cb200_heads& k, const cb200_heads& q_out,
+                                const cb200_heads& k_out, const cb200_qk_args& a, cb200_status* status,
+                                cudaStream_t stream);
+int64_t qk_backward_workspace(int dim);
+cudaError_t launch_qk_norm_rope_backward(const cb200_heads& grad_q, const cb200_heads& grad_k, const cb200_heads& q,
+                                         const cb200_heads& k, const cb200_heads& dq, const cb200_heads& dk,
+                                         float* dq_weight, float* dk_weight, const cb200_qk_args& a, void* workspace,
+                                         cb200_status* status, cudaStream_t stream);
+
 }  // namespace cb200

@@ -9,6 +9,10 @@
 """
 from __future__ import annotations
 
+import ctypes
+import struct
+from functools import lru_cache
+
 import torch
 
 from . import _cabi
@@ -429,3 +433,308 @@ def qembedding_route_rows(qtensor, ids: torch.Tensor, dst_ptrs, row_bounds, *, v
     _cabi.call("cb200_qembedding_route_rows", _ptr(qtensor.data), qtensor.dtype.value, _ptr(flat),
                ctypes.cast(arr, ctypes.c_void_p), len(ptrs), ctypes.cast(barr, ctypes.c_void_p), vocab, hidden,
                flat.shape[0], _ID_DTYPES[flat.dtype], begin, end, _ptr(status), _stream(flat))
+
+
+# ---- training and serving operators beside the path -------------------------------------------------
+# f32 inside with one rounding to the output's type; the sums of gradients are held in f32 and have a fixed
+# order, so equal inputs give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """The entry point `name` on `device`'s current stream, whichever device is current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _cabi.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _cabi.call(name, *args, stream)
+
+
+@lru_cache(maxsize=512)
+def _workspace_bytes(device: torch.device, name: str, *args) -> int:
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _cabi.call(name, *args, ctypes.addressof(n))
+    return n.value
+
+
+def _workspace(device: torch.device, name: str, *args) -> tuple[torch.Tensor, int]:
+    n = _workspace_bytes(device, name, *args)
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and one-past-last byte address of a tensor with non-negative strides."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views of one buffer, such as q and k of a packed projection, share no element: for a stride S that
+    both have and whose multiples all their larger strides are, their pieces lie apart within [0, S)."""
+    if a.dtype != b.dtype:
+        return False
+    size = a.element_size()
+    for step in set(a.stride()) & set(b.stride()):
+        inner = []
+        for t in (a, b):
+            dims = [(n, st) for n, st in zip(t.shape, t.stride()) if n > 1]
+            if any(st >= step and st % step for _, st in dims):
+                break
+            inner.append(1 + sum((n - 1) * st for n, st in dims if st < step))
+        at, rest = divmod((b.data_ptr() - a.data_ptr()) % (step * size), size) if step else (0, 1)
+        if len(inner) == 2 and rest == 0 and inner[0] <= at and at + inner[1] <= step:
+            return True
+    return False
+
+
+def _check_apart(op: str, out: torch.Tensor, *others: torch.Tensor | None, same: bool = True) -> None:
+    """Refuses an output that overlaps one of `others`, unless (with `same`) it is that very view."""
+    lo, hi = _span(out)
+    for t in others:
+        if t is None:
+            continue
+        a, b = _span(t)
+        if hi <= a or b <= lo:
+            continue
+        if same and t.data_ptr() == out.data_ptr() and t.stride() == out.stride() and t.shape == out.shape and t.dtype == out.dtype:
+            continue
+        if not _interleaved(out, t):
+            raise CandleError(f"the output of {op} overlaps another tensor of the call")
+
+
+def embedding_scaled(table: torch.Tensor, ids: torch.Tensor, scale: float, *, out: torch.Tensor | None = None,
+                     check: bool = True, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``scale * Embedding::forward(ids)`` in one launch, rounded once: the lookup of models that multiply the
+    embedding by a constant such as ``sqrt(hidden)``.  ids of any shape; the row of a bad id is left unwritten and
+    reported as by ``index_select``.  (candle multiplies in the table's type with the scale rounded to it.)"""
+    if table.dim() != 2 or not table.is_contiguous():
+        raise CandleError("index-select requires contiguous tensors")
+    if table.dtype not in _DTYPES:
+        raise CandleError(f"unsupported dtype {table.dtype} for embedding")
+    flat = _ids_checks(ids.reshape(-1))
+    _same_device(table, flat, out)
+    vocab, hidden = table.shape
+    final = [*ids.shape, hidden]
+    if out is None:
+        out = torch.empty(final, dtype=table.dtype, device=table.device)
+    else:
+        if list(out.shape) != final or out.dtype != table.dtype or not out.is_contiguous():
+            raise CandleError(f"out must be a contiguous tensor of shape {final}, got {_dims(out)}")
+        _check_apart("embedding", out, table, flat, same=False)
+    st = status if status is not None else (new_status(table.device) if check else None)
+    _launch(table.device, "cb200_embedding_scaled", _ptr(table), _ptr(flat), _ptr(out), vocab, hidden, flat.shape[0],
+            float(scale), _DTYPES[table.dtype], _ID_DTYPES[flat.dtype], _ptr(st))
+    if check:
+        raise_for_status(st)
+    return out
+
+
+def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float = 1.0,
+                       out: torch.Tensor | None = None, accumulate: bool = False, out_dtype: torch.dtype | None = None,
+                       padding_id: int | None = None, check: bool = True,
+                       status: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of ``scale * Embedding::forward(ids)`` with respect to the ``[vocab, hidden]`` table: row v is
+    ``scale`` times the sum of the rows of ``grad`` whose id is v, in f32 and in the order of the tokens.
+
+    ``grad`` is ``[*ids.shape, hidden]`` (rows may be strided).  The result is a fresh tensor of ``out_dtype``
+    (``grad``'s, or f32) or ``out``; every row is written, zeros where no id points.  With ``accumulate`` the sums are
+    added to ``out`` and the other rows are not touched.  Tokens whose id is ``padding_id`` contribute nothing."""
+    if grad.dtype not in _DTYPES:
+        raise CandleError(f"unsupported dtype {grad.dtype} for embedding-backward")
+    if grad.dim() == 0 or list(grad.shape[:-1]) != list(ids.shape):
+        raise CandleError(f"shape mismatch in embedding-backward {_dims(grad)} {_dims(ids)}")
+    hidden = grad.shape[-1]
+    flat = _ids_checks(ids.reshape(-1))
+    n = flat.shape[0]
+    try:
+        rows = grad.view(n, hidden)
+    except RuntimeError:
+        raise CandleError("the rows of grad must have one stride in embedding-backward") from None
+    if hidden > 1 and rows.stride(1) != 1:
+        raise CandleError("the last dimension of grad has to be contiguous in embedding-backward")
+    vocab = int(vocab)
+    if vocab < 0:
+        raise CandleError(f"the table of embedding-backward has {vocab} rows")
+    if out_dtype is None:
+        out_dtype = grad.dtype if out is None else out.dtype
+    if out_dtype != grad.dtype and out_dtype != torch.float32:
+        raise CandleError(f"unsupported dtype {out_dtype} for the result of embedding-backward of {grad.dtype}")
+    _same_device(grad, flat, out)
+    if out is None:
+        if accumulate:
+            raise CandleError("embedding-backward accumulates into `out`, which is missing")
+        out = torch.empty(vocab, hidden, dtype=out_dtype, device=grad.device)
+    else:
+        if list(out.shape) != [vocab, hidden] or out.dtype != out_dtype or not out.is_contiguous():
+            raise CandleError(f"out must be a contiguous {out_dtype} tensor of shape {[vocab, hidden]}, got {out.dtype} {_dims(out)}")
+        _check_apart("embedding-backward", out, rows, flat, same=False)
+    ws, ws_bytes = _workspace(grad.device, "cb200_embedding_backward_workspace", vocab, hidden, n)
+    st = status if status is not None else (new_status(grad.device) if check else None)
+    _launch(grad.device, "cb200_embedding_backward", _ptr(rows), rows.stride(0) if n > 1 else hidden, _ptr(flat), _ptr(out),
+            vocab, hidden, n, float(scale), -1 if padding_id is None else int(padding_id), 1 if accumulate else 0,
+            _DTYPES[grad.dtype], _DTYPES[out_dtype], _ID_DTYPES[flat.dtype], _ptr(ws), ws_bytes, _ptr(st))
+    if check:
+        raise_for_status(st)
+    return out
+
+
+def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor, eps: float, *,
+                      grad_sum: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """Gradient of ``rms_norm(xs, alpha, eps)``: ``(dxs, dalpha)`` for the gradient ``grad`` of its result, ``dalpha`` in
+    f32.  After ``rms_norm(x, alpha, eps, residual=r, return_sum=True)`` pass the returned sum as ``xs`` and the gradient
+    that reaches that sum on the residual stream as ``grad_sum``, which is added: ``dxs`` is then the gradient of both
+    ``x`` and ``r``.  ``out`` may be ``grad``, ``xs`` or ``grad_sum``."""
+    if xs.dim() == 0:
+        raise CandleError("unexpected rank, expected: at least 1, got: 0")
+    if alpha.dim() != 1:
+        raise CandleError(f"unexpected rank, expected: 1, got: {alpha.dim()} ({_dims(alpha)})")
+    if xs.shape[-1] != alpha.shape[0]:
+        raise CandleError(f"shape mismatch in rms-norm {_dims(xs)} {_dims(alpha)}")
+    for g in (grad, grad_sum):
+        if g is None:
+            continue
+        if g.shape != xs.shape or g.dtype != xs.dtype:
+            raise CandleError(f"shape mismatch in rms-norm-backward, xs: {_dims(xs)} {xs.dtype}, gradient: {_dims(g)} {g.dtype}")
+        if not g.is_contiguous():
+            raise CandleError("the gradient has to be contiguous")
+    _norm_checks("rms-norm", xs, [("alpha", alpha)], None)
+    _same_device(xs, grad, grad_sum)
+    dx = _out_check(out, xs)
+    if out is not None:
+        _check_apart("rms-norm-backward", out, grad, xs, grad_sum)
+        _check_apart("rms-norm-backward", out, alpha, same=False)
+    cols = xs.shape[-1]
+    rows = xs.numel() // cols if cols else 0
+    dalpha = torch.empty(cols, dtype=torch.float32, device=xs.device)
+    ws, ws_bytes = _workspace(xs.device, "cb200_rms_norm_backward_workspace", rows, cols)
+    _launch(xs.device, "cb200_rms_norm_backward", _ptr(grad), _ptr(xs), _ptr(alpha), _ptr(grad_sum), _ptr(dx), _ptr(dalpha),
+            rows, cols, float(eps), _DTYPES[xs.dtype], _ptr(ws), ws_bytes)
+    return dx, dalpha
+
+
+_HEADS = struct.Struct("=qqqqii")  # cb200_heads
+_QK_ARGS = struct.Struct("=qqqqqqqqiifiiiii")  # cb200_qk_args
+
+
+def _heads(t: torch.Tensor) -> bytes:
+    st = t.stride()
+    if t.dim() == 4:
+        return _HEADS.pack(t.data_ptr(), st[0], st[1], st[2], t.shape[2], 0)
+    return _HEADS.pack(t.data_ptr(), 0, st[0], st[1], t.shape[1], 0)
+
+
+def _qk_checks(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more=()) -> bytes:
+    """The checks that the head norms with rotation and their gradient share, and their arguments packed.  `more` are
+    tensors that have to be like q or k: (tensor, like)."""
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise CandleError(f"unexpected rank in {op}, expected: [tokens, heads, dim] or [batch, tokens, heads, dim], got: "
+                          f"{_dims(q)} {_dims(k)}")
+    d = q.shape[-1]
+    if k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]:
+        raise CandleError(f"shape mismatch in {op} {_dims(q)} {_dims(k)}")
+    if q.dtype not in _DTYPES or any(t.dtype != q.dtype for t in (k, q_weight, k_weight)):
+        raise CandleError(f"unsupported dtype for {op} {q.dtype} {k.dtype} {q_weight.dtype} {k_weight.dtype}")
+    for w in (q_weight, k_weight):
+        if w.dim() != 1 or w.shape[0] != d:
+            raise CandleError(f"shape mismatch in {op}, heads of {d} columns, weight: {_dims(w)}")
+        if not w.is_contiguous():
+            raise CandleError("the weight has to be contiguous")
+    if cos.dim() != 2 or sin.shape != cos.shape or not 0 < 2 * cos.shape[1] <= d:
+        raise CandleError(f"inconsistent last dim size in rope {_dims(q)} {_dims(cos)} {_dims(sin)}")
+    if not cos.is_contiguous():
+        raise CandleError("cos has to be contiguous in rope")
+    if not sin.is_contiguous():
+        raise CandleError("sin has to be contiguous in rope")
+    if sin.dtype != cos.dtype or cos.dtype not in (q.dtype, torch.float32):
+        raise CandleError(f"unsupported dtype for rope {q.dtype} {cos.dtype} {sin.dtype}")
+    for t, like in ((q, q), (k, k), *more):
+        if t.shape != like.shape or t.dtype != q.dtype:
+            raise CandleError(f"shape mismatch in {op} {_dims(like)} {like.dtype}, {_dims(t)} {t.dtype}")
+        if t.stride(-1) != 1 and d > 1:
+            raise CandleError(f"the last dimension has to be contiguous in {op}")
+    batch, tokens = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+    if positions is None:
+        if tokens > cos.shape[0]:
+            raise CandleError(f"inconsistent last dim size in rope {_dims(q)} {_dims(cos)} {_dims(sin)}")
+    else:
+        if positions.shape != q.shape[:-2]:
+            raise CandleError(f"shape mismatch in {op} {_dims(q)}, positions: {_dims(positions)}")
+        if positions.dtype not in _ID_DTYPES:
+            raise CandleError(f"unsupported dtype {positions.dtype} for positions (expected U8, U32 or I64)")
+        if not positions.is_contiguous():
+            raise CandleError(f"positions have to be contiguous in {op}")
+    _same_device(q, k, q_weight, k_weight, cos, sin, positions, *(t for t, _ in more))
+    return _QK_ARGS.pack(
+        q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        0 if positions is None else positions.data_ptr(), batch, tokens, cos.shape[0], d, 2 * cos.shape[1], eps,
+        1 if interleaved else 0, _DTYPES[q.dtype], _DTYPES[cos.dtype],
+        _cabi.ID_I64 if positions is None else _ID_DTYPES[positions.dtype], 0)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                 cos: torch.Tensor, sin: torch.Tensor, *, positions: torch.Tensor | None = None,
+                 interleaved: bool = False, out: tuple[torch.Tensor, torch.Tensor] | None = None, check: bool = True,
+                 status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head followed by its rotation, in one pass: ``rope(rms_norm(q, q_weight, eps))`` and
+    the same of k, computed in f32 and rounded once.
+
+    q is ``[batch, tokens, q_heads, dim]`` or ``[tokens, q_heads, dim]``, k the same with its own number of heads; any
+    strides but a contiguous last dimension, so views of a packed projection and ``[b, h, t, d]`` tensors seen through
+    ``transpose(1, 2)`` need no copy.  cos / sin are ``[positions, rotary / 2]`` in the heads' type or f32: the first
+    ``rotary`` columns are rotated, as ``rope`` does or (``interleaved``) as ``rope_i``.  ``positions`` has the shape of
+    the tokens; without it a token's position is its index in the sequence.  ``out`` may be (q, k) themselves.
+    The heads of a token whose position the tables do not have are left unwritten and reported."""
+    more = () if out is None else ((out[0], q), (out[1], k))
+    args = _qk_checks("qk-norm-rope", q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more)
+    if out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        q_out, k_out = out
+        _check_apart("qk-norm-rope", q_out, q)
+        _check_apart("qk-norm-rope", k_out, k)
+        _check_apart("qk-norm-rope", q_out, k, k_out, q_weight, k_weight, cos, sin, positions, same=False)
+        _check_apart("qk-norm-rope", k_out, q, q_weight, k_weight, cos, sin, positions, same=False)
+    check = check and positions is not None
+    st = status if status is not None else (new_status(q.device) if check else None)
+    _launch(q.device, "cb200_qk_norm_rope", _heads(q), _heads(k), _heads(q_out), _heads(k_out), args, _ptr(st))
+    if check:
+        raise_for_status(st, "qk-norm-rope")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float, cos: torch.Tensor,
+                          sin: torch.Tensor, *, positions: torch.Tensor | None = None, interleaved: bool = False,
+                          out: tuple[torch.Tensor, torch.Tensor] | None = None, check: bool = True,
+                          status: torch.Tensor | None = None):
+    """Gradient of ``qk_norm_rope``: ``(dq, dk, dq_weight, dk_weight)`` from the gradients of its two results and its
+    inputs (the same q, k, weights, cos, sin and positions), the weights' gradients in f32.  ``out`` receives (dq, dk)
+    and may be the gradients or (q, k) themselves."""
+    more = [(grad_q, q), (grad_k, k)]
+    if out is not None:
+        more += [(out[0], q), (out[1], k)]
+    op = "qk-norm-rope-backward"
+    args = _qk_checks(op, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more)
+    if out is None:
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        dq, dk = out
+        _check_apart(op, dq, q, grad_q)
+        _check_apart(op, dk, k, grad_k)
+        _check_apart(op, dq, k, grad_k, dk, q_weight, k_weight, cos, sin, positions, same=False)
+        _check_apart(op, dk, q, grad_q, q_weight, k_weight, cos, sin, positions, same=False)
+    dw = torch.empty(2, q.shape[-1], dtype=torch.float32, device=q.device)
+    ws, ws_bytes = _workspace(q.device, "cb200_qk_norm_rope_backward_workspace", q.shape[-1])
+    check = check and positions is not None
+    st = status if status is not None else (new_status(q.device) if check else None)
+    dq_weight, dk_weight = dw[0], dw[1]
+    _launch(q.device, "cb200_qk_norm_rope_backward", _heads(grad_q), _heads(grad_k), _heads(q), _heads(k), _heads(dq),
+            _heads(dk), _ptr(dq_weight), _ptr(dk_weight), args, _ptr(ws), ws_bytes, _ptr(st))
+    if check:
+        raise_for_status(st, op)
+    return dq, dk, dq_weight, dk_weight

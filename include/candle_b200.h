@@ -330,6 +330,110 @@ CB200_API int cb200_qembedding_route_rows(const void* qtable, int qtype, const v
                                 const int64_t* row_bounds, int64_t vocab, int32_t hidden, int64_t n_ids, int id_dtype,
                                 int64_t vocab_begin, int64_t vocab_end, cb200_status* status, cb200_stream_t stream);
 
+/*
+ * ---- Training and serving operators beside the path above (no counterpart in the reference, whose
+ * fused ops have no backward: CustomOp2/3 with `apply_op*_no_bwd`, candle-nn/src/ops.rs:651, 908).
+ * Their arithmetic is f32 inside with ONE rounding to the output's type; sums of gradients are held in
+ * f32 and taken in an order that depends on the shapes alone, so equal inputs give equal bits.
+ * Where a call needs scratch memory, `workspace` is device memory of at least the bytes that the
+ * matching *_workspace function reports, 16-byte aligned; it is written before it is read, holds
+ * nothing between calls, and two calls that may run at the same time need two of them.
+ */
+
+/*
+ * Scaled row lookup: out[i, :] = T(f32(table[ids[i], :]) * scale), for models that multiply the embedding by a
+ * constant such as sqrt(hidden).  candle multiplies in a launch of its own, with the constant rounded to T first;
+ * pass a scale that T represents for the same values.
+ * table [vocab, hidden], out [n_ids, hidden].  ids outside the table are reported through `status` and
+ * their rows left as they were.
+ */
+CB200_API int cb200_embedding_scaled(const void* table, const void* ids, void* out, int64_t vocab, int32_t hidden,
+                                     int64_t n_ids, float scale, int dtype, int id_dtype, cb200_status* status,
+                                     cb200_stream_t stream);
+
+/*
+ * Gradient of the (scaled) lookup with respect to the table:
+ *   out[v, :]  = T(scale * sum of grad[i, :] over the i with ids[i] == v)               accumulate == 0
+ *   out[v, :]  = T(out[v, :] + scale * that sum), rows that no id names left alone       accumulate != 0
+ * grad is [n_ids, hidden] with rows `grad_stride` elements apart (0 <= grad_stride; 0 is one row for all ids), out
+ * [vocab, hidden] of `out_dtype`: `dtype` or F32.  With accumulate == 0 every row of `out` is written (zeros
+ * where no id points).  Tokens whose id is `padding_id` contribute nothing (-1: there is none); ids outside
+ * the table contribute nothing and are reported.  `out` overlaps neither grad nor ids.
+ * The tokens are brought into the order of their ids (stable, so the sums have a fixed order).
+ * n_ids and vocab are below 2^31.
+ */
+CB200_API int cb200_embedding_backward(const void* grad, int64_t grad_stride, const void* ids, void* out, int64_t vocab,
+                                       int32_t hidden, int64_t n_ids, float scale, int64_t padding_id, int accumulate,
+                                       int dtype, int out_dtype, int id_dtype, void* workspace, int64_t workspace_bytes,
+                                       cb200_status* status, cb200_stream_t stream);
+CB200_API int cb200_embedding_backward_workspace(int64_t vocab, int32_t hidden, int64_t n_ids, int64_t* bytes);
+
+/*
+ * Gradient of cb200_rms_norm.  With r = 1 / sqrt(mean(x^2) + eps) of a row:
+ *   dx = T(r * (g * alpha - x * r^2 * mean(g * alpha * x)) + grad_sum),   dalpha = sum over rows of g * x * r
+ * x is what was normalised (with a residual: the sum that cb200_rms_norm returns in sum_out, and dx is then the
+ * gradient of both addends); grad_sum, the gradient that arrives at that sum by the residual stream, may be NULL.
+ * x, grad, grad_sum, dx: [rows, cols]; alpha [cols] of the same type; dalpha [cols] in F32, overwritten.  dx may be
+ * grad, x or grad_sum itself; partial overlap is not allowed.
+ */
+CB200_API int cb200_rms_norm_backward(const void* grad, const void* x, const void* alpha, const void* grad_sum, void* dx,
+                                      void* dalpha, int64_t rows, int32_t cols, float eps, int dtype, void* workspace,
+                                      int64_t workspace_bytes, cb200_stream_t stream);
+CB200_API int cb200_rms_norm_backward_workspace(int64_t rows, int32_t cols, int64_t* bytes);
+
+/*
+ * Queries or keys as [batch, tokens, heads, dim] with any strides (in elements) but a contiguous last dimension:
+ * a view of a packed projection, [b, t, h, d] or [b, h, t, d].
+ */
+typedef struct cb200_heads {
+  void* data;
+  int64_t batch_stride, token_stride, head_stride;
+  int32_t heads;
+  int32_t reserved;
+} cb200_heads;
+
+/* What cb200_qk_norm_rope and its gradient share. */
+typedef struct cb200_qk_args {
+  const void* q_weight;   /* [dim] of `dtype` */
+  const void* k_weight;   /* [dim] of `dtype` */
+  const void* cos;        /* [max_positions, rotary / 2] of `table_dtype` */
+  const void* sin;
+  const void* positions;  /* [batch, tokens] of `position_dtype`, or NULL: the index of the token in its sequence */
+  int64_t batch, tokens, max_positions;
+  int32_t dim, rotary;    /* the first `rotary` (even) columns of a head are rotated */
+  float eps;
+  int32_t interleaved;    /* pairs (x[2k], x[2k+1]) as rope_i, else (x[k], x[k + rotary/2]) as rope */
+  int32_t dtype;
+  int32_t table_dtype;    /* `dtype` or F32 */
+  int32_t position_dtype; /* CB200_ID_* */
+  int32_t reserved;
+} cb200_qk_args;
+
+/*
+ * RMS norm of every query and key head followed by its rotation, in one pass:
+ *   u = x / sqrt(mean(x^2) + eps) * weight;   out = T(rotation(position) u)
+ * the composition of cb200_rms_norm and cb200_rope without the roundings between them.  A position outside
+ * [0, max_positions) is reported through `status` and the token's heads are left as they were.  q_out / k_out
+ * may be q / k themselves (same strides); apart from that no output overlaps an input or another output.
+ * Either side may have zero heads.
+ */
+CB200_API int cb200_qk_norm_rope(const cb200_heads* q, const cb200_heads* k, const cb200_heads* q_out,
+                                 const cb200_heads* k_out, const cb200_qk_args* args, cb200_status* status,
+                                 cb200_stream_t stream);
+
+/*
+ * Its gradient.  With v = rotation^T g, r = 1 / sqrt(mean(x^2) + eps) of a head's row:
+ *   dx = T(r * (v * weight - x * r^2 * mean(v * weight * x))),   dweight = sum over tokens and heads of v * x * r
+ * q, k are the inputs of the forward call; dq_weight, dk_weight [dim] in F32, overwritten.  dq / dk may be
+ * grad_q / grad_k or q / k themselves (same strides).  Tokens with a bad position are reported, their dq / dk left as
+ * they were, and they add nothing to the weights' gradients.
+ */
+CB200_API int cb200_qk_norm_rope_backward(const cb200_heads* grad_q, const cb200_heads* grad_k, const cb200_heads* q,
+                                          const cb200_heads* k, const cb200_heads* dq, const cb200_heads* dk,
+                                          void* dq_weight, void* dk_weight, const cb200_qk_args* args, void* workspace,
+                                          int64_t workspace_bytes, cb200_status* status, cb200_stream_t stream);
+CB200_API int cb200_qk_norm_rope_backward_workspace(int32_t dim, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

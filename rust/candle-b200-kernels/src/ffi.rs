@@ -28,6 +28,40 @@ pub struct Cb200Status {
     pub size: i64,
 }
 
+/// `cb200_heads`: queries or keys `[batch, tokens, heads, dim]`, strides in elements.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Cb200Heads {
+    pub data: *mut c_void,
+    pub batch_stride: i64,
+    pub token_stride: i64,
+    pub head_stride: i64,
+    pub heads: i32,
+    pub reserved: i32,
+}
+
+/// `cb200_qk_args`
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Cb200QkArgs {
+    pub q_weight: *const c_void,
+    pub k_weight: *const c_void,
+    pub cos: *const c_void,
+    pub sin: *const c_void,
+    pub positions: *const c_void,
+    pub batch: i64,
+    pub tokens: i64,
+    pub max_positions: i64,
+    pub dim: i32,
+    pub rotary: i32,
+    pub eps: f32,
+    pub interleaved: i32,
+    pub dtype: i32,
+    pub table_dtype: i32,
+    pub position_dtype: i32,
+    pub reserved: i32,
+}
+
 extern "C" {
     pub fn cb200_version() -> c_int;
     pub fn cb200_last_error() -> *const c_char;
@@ -77,6 +111,25 @@ extern "C" {
     pub fn cb200_qembedding_route_rows(qtable: *const c_void, qtype: c_int, ids: *const c_void,
         dsts: *const *mut c_void, n_dsts: c_int, row_bounds: *const i64, vocab: i64, hidden: i32, n_ids: i64,
         id_dtype: c_int, vocab_begin: i64, vocab_end: i64, status: *mut Cb200Status, stream: *mut c_void) -> c_int;
+
+    pub fn cb200_embedding_scaled(table: *const c_void, ids: *const c_void, out: *mut c_void, vocab: i64, hidden: i32,
+        n_ids: i64, scale: f32, dtype: c_int, id_dtype: c_int, status: *mut Cb200Status, stream: *mut c_void) -> c_int;
+    pub fn cb200_embedding_backward(grad: *const c_void, grad_stride: i64, ids: *const c_void, out: *mut c_void,
+        vocab: i64, hidden: i32, n_ids: i64, scale: f32, padding_id: i64, accumulate: c_int, dtype: c_int,
+        out_dtype: c_int, id_dtype: c_int, workspace: *mut c_void, workspace_bytes: i64, status: *mut Cb200Status,
+        stream: *mut c_void) -> c_int;
+    pub fn cb200_embedding_backward_workspace(vocab: i64, hidden: i32, n_ids: i64, bytes: *mut i64) -> c_int;
+    pub fn cb200_rms_norm_backward(grad: *const c_void, x: *const c_void, alpha: *const c_void,
+        grad_sum: *const c_void, dx: *mut c_void, dalpha: *mut c_void, rows: i64, cols: i32, eps: f32, dtype: c_int,
+        workspace: *mut c_void, workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn cb200_rms_norm_backward_workspace(rows: i64, cols: i32, bytes: *mut i64) -> c_int;
+    pub fn cb200_qk_norm_rope(q: *const Cb200Heads, k: *const Cb200Heads, q_out: *const Cb200Heads,
+        k_out: *const Cb200Heads, args: *const Cb200QkArgs, status: *mut Cb200Status, stream: *mut c_void) -> c_int;
+    pub fn cb200_qk_norm_rope_backward(grad_q: *const Cb200Heads, grad_k: *const Cb200Heads, q: *const Cb200Heads,
+        k: *const Cb200Heads, dq: *const Cb200Heads, dk: *const Cb200Heads, dq_weight: *mut c_void,
+        dk_weight: *mut c_void, args: *const Cb200QkArgs, workspace: *mut c_void, workspace_bytes: i64,
+        status: *mut Cb200Status, stream: *mut c_void) -> c_int;
+    pub fn cb200_qk_norm_rope_backward_workspace(dim: i32, bytes: *mut i64) -> c_int;
 }
 
 #[cfg(feature = "nccl")]
