@@ -163,8 +163,8 @@ int check_qk(const char* name, const cb200_qk_args* a) {
   if (a->positions != nullptr && !valid_id_dtype(a->position_dtype))
     return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported positions dtype code %d", name, a->position_dtype);
   if (a->batch < 0 || a->tokens < 0 || a->max_positions < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape", name);
-  if (a->batch > (int64_t(1) << 31) || a->tokens > (int64_t(1) << 31) || a->batch * a->tokens > (int64_t(1) << 31))
-    return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: more than 2^31 tokens", name);
+  if (a->batch >= (int64_t(1) << 31) || a->tokens >= (int64_t(1) << 31) || a->batch * a->tokens >= (int64_t(1) << 31))
+    return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: 2^31 tokens or more", name);
   if (a->dim <= 0 || a->rotary <= 0 || a->rotary > a->dim || a->rotary % 2 != 0)
     return fail(CB200_E_INVALID_ARGUMENT, "%s: %d rotated columns of %d (expected an even number of at most the head size)", name,
                 a->rotary, a->dim);

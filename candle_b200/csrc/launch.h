@@ -151,8 +151,9 @@ struct RmsBackwardArgs {
 };
 int64_t rms_backward_workspace(int64_t rows, int n);
 cudaError_t launch_rms_backward(int dtype, const RmsBackwardArgs& a, void* workspace, cudaStream_t stream);
-// out[c] = sum over p of partials[p * cols + c], in the order of p within fixed groups (rms_backward.cu)
-cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, cudaStream_t stream);
+// Sum over p of partials[p * cols + c] in a fixed order, to out[c] for c < split, out2[c - split] behind (rms_backward.cu)
+cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, int split, float* out2,
+                                cudaStream_t stream);
 
 // Head norms with the rotation in the same pass (head_norm.cu)
 cudaError_t launch_qk_norm_rope(const cb200_heads& q, const cb200_heads& k, const cb200_heads& q_out,

@@ -79,23 +79,220 @@ __global__ void __launch_bounds__(kThreads) dx_kernel(const RmsBackwardArgs a, c
   }
 }
 
-// 32 columns per CTA, its eight warps over the partial rows.
-__global__ void __launch_bounds__(256) sum_partials_kernel(const float* partials, int n_partials, int cols, float* out) {
-  __shared__ float part[8][32];
+// 32 columns per CTA, its warps over the partial rows: warp w takes rows w, w + 32, ... and the warps' sums are added
+// in order.  Columns from `split` on go to out2.
+constexpr int kSumWarps = 32;
+__global__ void __launch_bounds__(kSumWarps * 32) sum_partials_kernel(const float* partials, int n_partials, int cols,
+                                                                      float* out, int split, float* out2) {
+  __shared__ float part[kSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float acc = 0.0f;
-  if (c < cols)
-    for (int p = warp; p < n_partials; p += 8) acc += partials[static_cast<int64_t>(p) * cols + c];
+  if (c < cols) {
+#pragma unroll 4
+    for (int p = warp; p < n_partials; p += kSumWarps) acc += partials[static_cast<int64_t>(p) * cols + c];
+  }
   part[warp][lane] = acc;
   __syncthreads();
-  if (warp == 0 && c < cols) {
-    for (int w = 1; w < 8; ++w) acc += part[w][lane];
-    out[c] = acc;
+  // warp w adds up column w: lane k holds the sum of warp k
+  const float sum = warp_sum(part[lane][warp]);
+  const int column = blockIdx.x * 32 + warp;
+  if (lane == 0 && column < cols) {
+    if (column < split) out[column] = sum;
+    else out2[column - split] = sum;
   }
 }
 
-int max_partials() { return 2 * sm_count(); }
+int max_partials() { return 4 * sm_count(); }
+
+// ---- whole 16-byte vectors: one pass -----------------------------------------------------------------------------
+// TPR threads take a row, VPT vectors each (columns fixed per thread, so dalpha accumulates in registers); a CTA works on
+// kThreads / TPR rows at a time and walks over the rows persistently.  Every thread brings its own vectors of the rows
+// to come into its own slots of shared memory by asynchronous copies, kStages - 1 rows ahead, and reads back only
+// what it copied itself: no barrier guards the ring, and the only one per row is that of the row sums (none for rows
+// of up to 32 threads).
+template <int VPT>
+struct Ring {
+  static constexpr int kStages = VPT >= 3 ? 2 : 4;
+};
+
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+struct FastArgs {
+  RmsBackwardArgs a;
+  float* partials;  // [grid][n]
+  int tpr_shift, V;
+};
+
+constexpr int kScratchBytes = 2 * kThreads / 32 * 8;
+
+template <int DT, int VPT, bool SUM>
+__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  constexpr int P2 = Elem<DT>::kPerVec / 2, kInputs = SUM ? 3 : 2, kStages = Ring<VPT>::kStages;
+  float2* scratch = reinterpret_cast<float2*>(shared);             // [2][warps]
+  uint4* ring = reinterpret_cast<uint4*>(shared + kScratchBytes);  // [stage][input][vector][thread]
+  const RmsBackwardArgs& a = f.a;
+  const int tpr = 1 << f.tpr_shift, sub = threadIdx.x >> f.tpr_shift, at0 = threadIdx.x & (tpr - 1);
+  const int rows_at_once = kThreads >> f.tpr_shift;
+  const int V = f.V;
+  const float inv_n = 1.0f / static_cast<float>(a.n);
+  const uint4* src[3] = {static_cast<const uint4*>(a.x), static_cast<const uint4*>(a.grad), static_cast<const uint4*>(a.grad_sum)};
+  const int64_t n_tiles = (a.rows + rows_at_once - 1) / rows_at_once;
+
+  auto fetch = [&](int64_t tile, int stage) {
+    const int64_t row = tile * rows_at_once + sub;
+    if (row < a.rows) {
+#pragma unroll
+      for (int i = 0; i < kInputs; ++i)
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+          if (at0 + k * tpr < V)
+            cp_async16(&ring[((stage * kInputs + i) * VPT + k) * kThreads + threadIdx.x], src[i] + row * V + at0 + k * tpr);
+    }
+    cp_async_commit();
+  };
+
+  F2 acc[VPT][P2];
+  uint4 w[VPT];
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    w[k] = at0 + k * tpr < V ? __ldg(static_cast<const uint4*>(a.alpha) + at0 + k * tpr) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < P2; ++j) acc[k][j] = 0;
+  }
+
+  int64_t ahead = blockIdx.x;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    fetch(ahead, s);
+    ahead += gridDim.x;
+  }
+  int stage = 0, turn = 0;
+  for (int64_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+    fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);
+    ahead += gridDim.x;
+    copies_wait<kStages - 1>();
+    const uint4* slot = ring + stage * kInputs * VPT * kThreads + threadIdx.x;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    const int64_t row = tile * rows_at_once + sub;
+    const bool live = row < a.rows;
+    F2 xx = 0, gax = 0;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      if (!live || at0 + k * tpr >= V) continue;
+      F2 x[P2], g[P2], u[P2];
+      vec_to_pairs<DT>(slot[k * kThreads], x);
+      vec_to_pairs<DT>(slot[(VPT + k) * kThreads], g);
+      vec_to_pairs<DT>(w[k], u);
+#pragma unroll
+      for (int j = 0; j < P2; ++j) {
+        xx = fma2(x[j], x[j], xx);
+        gax = fma2(mul2(g[j], u[j]), x[j], gax);
+      }
+    }
+    const float2 t1 = unpair(xx), t2 = unpair(gax);
+    float2 sums = make_float2(t1.x + t1.y, t2.x + t2.y);
+    for (int o = tpr < 32 ? tpr >> 1 : 16; o > 0; o >>= 1) {
+      sums.x += __shfl_xor_sync(0xFFFFFFFFu, sums.x, o);
+      sums.y += __shfl_xor_sync(0xFFFFFFFFu, sums.y, o);
+    }
+    if (tpr > 32) {
+      if ((threadIdx.x & 31) == 0) scratch[turn + (threadIdx.x >> 5)] = sums;
+      __syncthreads();
+      const int warps = tpr >> 5, first = sub * warps;
+      sums = make_float2(0.0f, 0.0f);
+      for (int i = 0; i < warps; ++i) {
+        sums.x += scratch[turn + first + i].x;
+        sums.y += scratch[turn + first + i].y;
+      }
+      turn ^= kThreads / 32;  // the next row's sums go elsewhere: a thread may still be reading these
+    }
+    const float r = rsqrtf(fmaf(sums.x, inv_n, a.eps));
+    const float along = -r * (r * (r * (sums.y * inv_n)));
+    const F2 r2 = pair(r, r), along2 = pair(along, along);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      if (!live || at0 + k * tpr >= V) continue;
+      F2 x[P2], g[P2], u[P2];
+      vec_to_pairs<DT>(slot[k * kThreads], x);
+      vec_to_pairs<DT>(slot[(VPT + k) * kThreads], g);
+      vec_to_pairs<DT>(w[k], u);
+      F2 d[P2];
+#pragma unroll
+      for (int j = 0; j < P2; ++j) {
+        const F2 gr = mul2(g[j], r2);
+        acc[k][j] = fma2(gr, x[j], acc[k][j]);
+        d[j] = fma2(gr, u[j], mul2(x[j], along2));
+      }
+      if constexpr (SUM) {
+        F2 e[P2];
+        vec_to_pairs<DT>(slot[(2 * VPT + k) * kThreads], e);
+#pragma unroll
+        for (int j = 0; j < P2; ++j) d[j] = add2(d[j], e[j]);
+      }
+      stg_stream(static_cast<uint4*>(a.dx) + row * V + at0 + k * tpr, pairs_to_vec<DT>(d));
+    }
+  }
+
+  // the rows' groups of this CTA, added through shared memory (the ring is idle now): [group][n]
+  __syncthreads();
+  float* line = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    if (at0 + k * tpr >= V) continue;
+#pragma unroll
+    for (int j = 0; j < P2; ++j)
+      *reinterpret_cast<F2*>(line + sub * a.n + (at0 + k * tpr) * 2 * P2 + 2 * j) = acc[k][j];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.n; c += kThreads) {
+    float t = line[c];
+    for (int i = 1; i < rows_at_once; ++i) t += line[i * a.n + c];
+    f.partials[static_cast<int64_t>(blockIdx.x) * a.n + c] = t;
+  }
+}
+
+template <int DT, int VPT, bool SUM>
+cudaError_t launch_rows(const FastArgs& f, cudaStream_t stream) {
+  auto kern = rows_kernel<DT, VPT, SUM>;
+  const size_t input = static_cast<size_t>(Ring<VPT>::kStages) * VPT * kThreads * 16;
+  const size_t smem = kScratchBytes + input * (SUM ? 3 : 2);
+  cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), kThreads, smem, -1, nullptr);
+  if (e != cudaSuccess) return e;
+  // with and without grad_sum the same grid, so that dalpha is summed in the same order
+  int per_sm = 1;
+  e = kernel_launch_config(reinterpret_cast<const void*>(rows_kernel<DT, VPT, true>), kThreads, kScratchBytes + input * 3, -1, &per_sm);
+  if (e != cudaSuccess) return e;
+  const int rows_at_once = kThreads >> f.tpr_shift;
+  int64_t grid = static_cast<int64_t>(sm_count()) * per_sm;
+  if (grid > max_partials()) grid = max_partials();
+  const int64_t tiles = (f.a.rows + rows_at_once - 1) / rows_at_once;
+  if (grid > tiles) grid = tiles;
+  kern<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f);
+  e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_sum_partials(f.partials, static_cast<int>(grid), f.a.n, f.a.dalpha, f.a.n, nullptr, stream);
+}
+
+// The fewest threads per row (8 .. 256) that leave at most four vectors to each; false: the row is too long.
+template <int DT>
+bool launch_fast(const RmsBackwardArgs& a, float* partials, cudaStream_t stream, cudaError_t* e) {
+  FastArgs f{a, partials, 3, a.n / Elem<DT>::kPerVec};
+  while (f.tpr_shift < 8 && (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift > 4) ++f.tpr_shift;
+  const int vpt = (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift;
+  if (vpt > 4) return false;
+  const bool sum = a.grad_sum != nullptr;
+  switch (vpt) {
+    case 1: *e = sum ? launch_rows<DT, 1, true>(f, stream) : launch_rows<DT, 1, false>(f, stream); break;
+    case 2: *e = sum ? launch_rows<DT, 2, true>(f, stream) : launch_rows<DT, 2, false>(f, stream); break;
+    case 3: *e = sum ? launch_rows<DT, 3, true>(f, stream) : launch_rows<DT, 3, false>(f, stream); break;
+    default: *e = sum ? launch_rows<DT, 4, true>(f, stream) : launch_rows<DT, 4, false>(f, stream); break;
+  }
+  return true;
+}
 
 template <int DT>
 cudaError_t launch_any(const RmsBackwardArgs& a, float* partials, float2* factors, cudaStream_t stream) {
@@ -107,13 +304,14 @@ cudaError_t launch_any(const RmsBackwardArgs& a, float* partials, float2* factor
   alpha_partials_kernel<DT><<<blocks, kThreads, 0, stream>>>(a, factors, partials);
   dx_kernel<DT><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a, factors);
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_sum_partials(partials, slices, a.n, a.dalpha, stream);
+  return e != cudaSuccess ? e : launch_sum_partials(partials, slices, a.n, a.dalpha, a.n, nullptr, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, cudaStream_t stream) {
-  sum_partials_kernel<<<(cols + 31) / 32, 256, 0, stream>>>(partials, n_partials, cols, out);
+cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, int split, float* out2,
+                                cudaStream_t stream) {
+  sum_partials_kernel<<<(cols + 31) / 32, kSumWarps * 32, 0, stream>>>(partials, n_partials, cols, out, split, out2);
   return cudaGetLastError();
 }
 
@@ -127,10 +325,14 @@ cudaError_t launch_rms_backward(int dtype, const RmsBackwardArgs& a, void* works
   float* partials = static_cast<float*>(workspace);
   float2* factors = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
                                               ((static_cast<int64_t>(max_partials()) * a.n * 4 + 15) & ~int64_t(15)));
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.alpha) |
+                       reinterpret_cast<uintptr_t>(a.grad_sum) | reinterpret_cast<uintptr_t>(a.dx);
+  const bool vectors = at % 16 == 0 && a.n % (dtype == kDtF32 ? 4 : 8) == 0;
+  cudaError_t e = cudaSuccess;
   switch (dtype) {
-    case kDtF32: return launch_any<kDtF32>(a, partials, factors, stream);
-    case kDtF16: return launch_any<kDtF16>(a, partials, factors, stream);
-    default: return launch_any<kDtBF16>(a, partials, factors, stream);
+    case kDtF32: return vectors && launch_fast<kDtF32>(a, partials, stream, &e) ? e : launch_any<kDtF32>(a, partials, factors, stream);
+    case kDtF16: return vectors && launch_fast<kDtF16>(a, partials, stream, &e) ? e : launch_any<kDtF16>(a, partials, factors, stream);
+    default: return vectors && launch_fast<kDtBF16>(a, partials, stream, &e) ? e : launch_any<kDtBF16>(a, partials, factors, stream);
   }
 }
 

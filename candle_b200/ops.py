@@ -440,14 +440,24 @@ def qembedding_route_rows(qtensor, ids: torch.Tensor, dst_ptrs, row_bounds, *, v
 # order, so equal inputs give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
 
 
+def _stream_of(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The current stream's handle without a Stream object around it: a launch of a few microseconds feels the difference.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is not None:
+    def _stream_of(device: torch.device) -> int:  # noqa: F811
+        return _raw_stream(device.index)
+
+
 def _launch(device: torch.device, name: str, *args) -> None:
     """The entry point `name` on `device`'s current stream, whichever device is current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
     if device.index == torch.cuda.current_device():
-        _cabi.call(name, *args, stream)
+        _cabi.call(name, *args, _stream_of(device))
     else:
         with torch.cuda.device(device):
-            _cabi.call(name, *args, stream)
+            _cabi.call(name, *args, _stream_of(device))
 
 
 @lru_cache(maxsize=512)
@@ -619,16 +629,16 @@ _HEADS = struct.Struct("=qqqqii")  # cb200_heads
 _QK_ARGS = struct.Struct("=qqqqqqqqiifiiiii")  # cb200_qk_args
 
 
-def _heads(t: torch.Tensor) -> bytes:
-    st = t.stride()
-    if t.dim() == 4:
-        return _HEADS.pack(t.data_ptr(), st[0], st[1], st[2], t.shape[2], 0)
-    return _HEADS.pack(t.data_ptr(), 0, st[0], st[1], t.shape[1], 0)
+def _heads(t: torch.Tensor, rank: int, heads: int) -> bytes:
+    if rank == 4:
+        batch, token, head, _ = t.stride()
+        return _HEADS.pack(t.data_ptr(), batch, token, head, heads, 0)
+    token, head, _ = t.stride()
+    return _HEADS.pack(t.data_ptr(), 0, token, head, heads, 0)
 
 
-def _qk_checks(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more=()) -> bytes:
-    """The checks that the head norms with rotation and their gradient share, and their arguments packed.  `more` are
-    tensors that have to be like q or k: (tensor, like)."""
+def _qk_refuse(op: str, q, k, q_weight, k_weight, cos, sin, positions, more) -> None:
+    """Raises what is wrong with the arguments of the head norms with rotation or their gradient."""
     if q.dim() not in (3, 4) or k.dim() != q.dim():
         raise CandleError(f"unexpected rank in {op}, expected: [tokens, heads, dim] or [batch, tokens, heads, dim], got: "
                           f"{_dims(q)} {_dims(k)}")
@@ -655,9 +665,8 @@ def _qk_checks(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, inte
             raise CandleError(f"shape mismatch in {op} {_dims(like)} {like.dtype}, {_dims(t)} {t.dtype}")
         if t.stride(-1) != 1 and d > 1:
             raise CandleError(f"the last dimension has to be contiguous in {op}")
-    batch, tokens = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
     if positions is None:
-        if tokens > cos.shape[0]:
+        if q.shape[-3] > cos.shape[0]:
             raise CandleError(f"inconsistent last dim size in rope {_dims(q)} {_dims(cos)} {_dims(sin)}")
     else:
         if positions.shape != q.shape[:-2]:
@@ -667,11 +676,35 @@ def _qk_checks(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, inte
         if not positions.is_contiguous():
             raise CandleError(f"positions have to be contiguous in {op}")
     _same_device(q, k, q_weight, k_weight, cos, sin, positions, *(t for t, _ in more))
-    return _QK_ARGS.pack(
+
+
+def _qk_args(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more=()):
+    """The checked arguments that the head norms with rotation and their gradient share, packed, and (rank, q heads,
+    k heads, dim, device).  `more` are tensors that have to be like q or k: (tensor, like).  What is right is decided
+    by one chain of comparisons, since a decoding step's kernel takes less time than its checks; `_qk_refuse` then
+    says what is wrong."""
+    qs, ks, cs, t, ct, dev = q.shape, k.shape, cos.shape, q.dtype, cos.dtype, q.get_device()
+    rank = len(qs)
+    if not (
+        (rank == 4 or rank == 3) and len(ks) == rank and len(cs) == 2 and sin.shape == cs
+        and qs[-1] == ks[-1] and qs[:-2] == ks[:-2] and 0 < 2 * cs[1] <= qs[-1]
+        and t in _DTYPES and k.dtype == t and q_weight.dtype == t and k_weight.dtype == t
+        and (ct == t or ct == torch.float32) and sin.dtype == ct
+        and q_weight.shape == k_weight.shape == (qs[-1],)
+        and q_weight.is_contiguous() and k_weight.is_contiguous() and cos.is_contiguous() and sin.is_contiguous()
+        and q.stride(-1) == 1 and k.stride(-1) == 1
+        and all(m.shape == like.shape and m.dtype == t and m.get_device() == dev and m.stride(-1) == 1 for m, like in more)
+        and (qs[-3] <= cs[0] if positions is None else positions.shape == qs[:-2] and positions.dtype in _ID_DTYPES
+             and positions.is_contiguous() and positions.get_device() == dev)
+        and dev >= 0 and k.get_device() == dev and q_weight.get_device() == dev and k_weight.get_device() == dev
+        and cos.get_device() == dev and sin.get_device() == dev
+    ):
+        _qk_refuse(op, q, k, q_weight, k_weight, cos, sin, positions, more)
+    args = _QK_ARGS.pack(
         q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-        0 if positions is None else positions.data_ptr(), batch, tokens, cos.shape[0], d, 2 * cos.shape[1], eps,
-        1 if interleaved else 0, _DTYPES[q.dtype], _DTYPES[cos.dtype],
-        _cabi.ID_I64 if positions is None else _ID_DTYPES[positions.dtype], 0)
+        0 if positions is None else positions.data_ptr(), qs[0] if rank == 4 else 1, qs[-3], cs[0], qs[-1], 2 * cs[1], eps,
+        1 if interleaved else 0, _DTYPES[t], _DTYPES[ct], _cabi.ID_I64 if positions is None else _ID_DTYPES[positions.dtype], 0)
+    return args, rank, qs[-2], ks[-2], qs[-1], q.device
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
@@ -688,10 +721,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     the tokens; without it a token's position is its index in the sequence.  ``out`` may be (q, k) themselves.
     The heads of a token whose position the tables do not have are left unwritten and reported."""
     more = () if out is None else ((out[0], q), (out[1], k))
-    args = _qk_checks("qk-norm-rope", q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more)
+    args, rank, q_heads, k_heads, _, device = _qk_args("qk-norm-rope", q, k, q_weight, k_weight, eps, cos, sin, positions,
+                                                       interleaved, more)
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
     else:
         q_out, k_out = out
         _check_apart("qk-norm-rope", q_out, q)
@@ -699,8 +732,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         _check_apart("qk-norm-rope", q_out, k, k_out, q_weight, k_weight, cos, sin, positions, same=False)
         _check_apart("qk-norm-rope", k_out, q, q_weight, k_weight, cos, sin, positions, same=False)
     check = check and positions is not None
-    st = status if status is not None else (new_status(q.device) if check else None)
-    _launch(q.device, "cb200_qk_norm_rope", _heads(q), _heads(k), _heads(q_out), _heads(k_out), args, _ptr(st))
+    st = status if status is not None else (new_status(device) if check else None)
+    _launch(device, "cb200_qk_norm_rope", _heads(q, rank, q_heads), _heads(k, rank, k_heads), _heads(q_out, rank, q_heads),
+            _heads(k_out, rank, k_heads), args, _ptr(st))
     if check:
         raise_for_status(st, "qk-norm-rope")
     return q_out, k_out
@@ -718,23 +752,24 @@ def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.T
     if out is not None:
         more += [(out[0], q), (out[1], k)]
     op = "qk-norm-rope-backward"
-    args = _qk_checks(op, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved, more)
+    args, rank, q_heads, k_heads, dim, device = _qk_args(op, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved,
+                                                         more)
     if out is None:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     else:
         dq, dk = out
         _check_apart(op, dq, q, grad_q)
         _check_apart(op, dk, k, grad_k)
         _check_apart(op, dq, k, grad_k, dk, q_weight, k_weight, cos, sin, positions, same=False)
         _check_apart(op, dk, q, grad_q, q_weight, k_weight, cos, sin, positions, same=False)
-    dw = torch.empty(2, q.shape[-1], dtype=torch.float32, device=q.device)
-    ws, ws_bytes = _workspace(q.device, "cb200_qk_norm_rope_backward_workspace", q.shape[-1])
+    dw = torch.empty(2, dim, dtype=torch.float32, device=device)
+    ws, ws_bytes = _workspace(device, "cb200_qk_norm_rope_backward_workspace", dim)
     check = check and positions is not None
-    st = status if status is not None else (new_status(q.device) if check else None)
-    dq_weight, dk_weight = dw[0], dw[1]
-    _launch(q.device, "cb200_qk_norm_rope_backward", _heads(grad_q), _heads(grad_k), _heads(q), _heads(k), _heads(dq),
-            _heads(dk), _ptr(dq_weight), _ptr(dk_weight), args, _ptr(ws), ws_bytes, _ptr(st))
+    st = status if status is not None else (new_status(device) if check else None)
+    dq_weight, dk_weight = dw.unbind(0)
+    _launch(device, "cb200_qk_norm_rope_backward", _heads(grad_q, rank, q_heads), _heads(grad_k, rank, k_heads),
+            _heads(q, rank, q_heads), _heads(k, rank, k_heads), _heads(dq, rank, q_heads), _heads(dk, rank, k_heads),
+            _ptr(dq_weight), _ptr(dk_weight), args, _ptr(ws), ws_bytes, _ptr(st))
     if check:
         raise_for_status(st, op)
     return dq, dk, dq_weight, dk_weight
