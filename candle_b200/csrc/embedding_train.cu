@@ -1,14 +1,15 @@
 // The scaled lookup and the gradient of the embedding table.
 //
 // Gradient: out[v] = scale * sum of grad[i] over the tokens i with ids[i] == v.  The tokens are sorted by id
-// (stable radix sort of (id, position) pairs), so each table row owns a contiguous run of the sorted list and
-// its sum has a fixed order: no floating-point atomics, equal inputs give equal bits.  Then
+// (stable, as (id, position) pairs), so each table row owns a contiguous run of the sorted list and its sum has a
+// fixed order: no floating-point atomics, equal inputs give equal bits.  Then
 //   - chunk_sums_kernel adds up every aligned chunk of 32 sorted tokens that belongs to one id: text is skewed
 //     (the hottest id of 65536 tokens has thousands) and this is what spreads a long run over the GPU;
 //   - row_sums_kernel writes the table rows.  Work is cut by tokens, not by rows, since a few rows of a text's table
 //     have most of its tokens: a warp adds the runs that begin at a few neighbouring sorted positions, a CTA a
 //     long run (the chunk sums and the ends that do not fill a chunk).
-// The rows without tokens are filled with zeros beside the sort, whose few CTAs leave the memory idle.
+// The rows without tokens are filled with zeros by further blocks of the sort's launches, which leave the memory idle, or
+// where the sort takes less than a launch's time by blocks of row_stream_kernel.
 #include "launch.h"
 
 namespace cb200 {
@@ -17,17 +18,31 @@ namespace {
 
 bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// VEC consecutive elements <-> floats; VEC is the 16-byte vector's element count or 1 (any alignment).
+// One VEC-element unit as it lies in memory.
 template <int DT, int VEC>
-__device__ __forceinline__ void load_floats(const void* base, int64_t elem, float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    f[0] = load_elem<DT>(base, elem);
-  } else {
-    static_assert(VEC == Elem<DT>::kPerVec, "one 16-byte vector");
-    vec_to_floats<DT>(ldg_stream(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + elem * Elem<DT>::kBytes)), f);
-  }
+struct Unit {
+  uint4 v;
+};
+template <int DT>
+struct Unit<DT, 1> {
+  float v;
+};
+template <int DT, int VEC>
+__device__ __forceinline__ Unit<DT, VEC> load_unit(const void* base, int64_t elem) {
+  Unit<DT, VEC> u;
+  if constexpr (VEC == 1) u.v = load_elem<DT>(base, elem);
+  else u.v = ldg_stream(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + elem * Elem<DT>::kBytes));
+  return u;
 }
-// As load_floats, for memory that this launch also writes (no read-only path).
+// f = the unit's elements times `scale`, each rounded once in f32.
+template <int DT, int VEC>
+__device__ __forceinline__ void scale_unit(const Unit<DT, VEC>& u, float scale, float (&f)[VEC]) {
+  if constexpr (VEC == 1) f[0] = u.v;
+  else vec_to_floats<DT>(u.v, f);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) f[i] = __fmul_rn(f[i], scale);
+}
+// VEC consecutive elements <-> floats; VEC is the 16-byte vector's element count of one of the types, or 1 (any alignment).
 template <int DT, int VEC>
 __device__ __forceinline__ void load_floats_plain(const void* base, int64_t elem, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
@@ -62,45 +77,71 @@ __device__ __forceinline__ void store_floats(void* base, int64_t elem, const flo
 }
 
 // ---------------------------------------------------------------------------------------------
-// Scaled lookup: a warp per (token, tile of columns)
+// Scaled lookup: a warp per (token, tile of 32 U units), its loads in flight together
 // ---------------------------------------------------------------------------------------------
-template <int DT, int VEC>
+template <int DT, int VEC, int U>
 __global__ void __launch_bounds__(256) scaled_lookup_kernel(const ScaledLookupArgs a, int units, int tiles) {
   const int lane = threadIdx.x & 31;
   const int64_t n_warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
   const int64_t n_items = a.n_ids * tiles;
   for (int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; item < n_items; item += n_warps) {
     const int64_t i = item / tiles;
-    const int u = static_cast<int>(item - i * tiles) * 32 + lane;
+    const int u0 = static_cast<int>(item - i * tiles) * (32 * U) + lane;
     const uint64_t id = read_id(a.ids, a.id_dtype, i);
     if (id >= static_cast<uint64_t>(a.vocab)) {
-      if (u == 0) report_status(a.status, CB200_STATUS_INVALID_INDEX, i, static_cast<int64_t>(id), a.vocab);
+      if (u0 == 0) report_status(a.status, CB200_STATUS_INVALID_INDEX, i, static_cast<int64_t>(id), a.vocab);
       continue;
     }
-    if (u >= units) continue;
-    float f[VEC];
-    load_floats<DT, VEC>(a.table, static_cast<int64_t>(id) * a.hidden + static_cast<int64_t>(u) * VEC, f);
+    Unit<DT, VEC> q[U];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = __fmul_rn(f[e], a.scale);
-    store_floats<DT, VEC>(a.out, i * a.hidden + static_cast<int64_t>(u) * VEC, f);
+    for (int k = 0; k < U; ++k)
+      if (u0 + 32 * k < units)
+        q[k] = load_unit<DT, VEC>(a.table, static_cast<int64_t>(id) * a.hidden + static_cast<int64_t>(u0 + 32 * k) * VEC);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (u0 + 32 * k >= units) continue;
+      float f[VEC];
+      scale_unit<DT, VEC>(q[k], a.scale, f);
+      store_floats<DT, VEC>(a.out, i * a.hidden + static_cast<int64_t>(u0 + 32 * k) * VEC, f);
+    }
   }
 }
 
-template <int DT, int VEC>
+template <int DT, int VEC, int U>
 cudaError_t launch_scaled_lookup_t(const ScaledLookupArgs& a, cudaStream_t stream) {
-  const int units = a.hidden / VEC, tiles = (units + 31) / 32;
+  const int units = a.hidden / VEC, tiles = (units + 32 * U - 1) / (32 * U);
   int64_t grid = (a.n_ids * tiles + 7) / 8;
-  const int64_t cap = static_cast<int64_t>(sm_count()) * 32;
+  const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
   if (grid > cap) grid = cap;
-  scaled_lookup_kernel<DT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, units, tiles);
+  scaled_lookup_kernel<DT, VEC, U><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, units, tiles);
   return cudaGetLastError();
 }
 
 template <int DT>
 cudaError_t launch_scaled_lookup_dt(const ScaledLookupArgs& a, cudaStream_t stream) {
   constexpr int kPV = Elem<DT>::kPerVec;
-  if (a.hidden % kPV == 0 && aligned_to(a.table, 16) && aligned_to(a.out, 16)) return launch_scaled_lookup_t<DT, kPV>(a, stream);
-  return launch_scaled_lookup_t<DT, 1>(a, stream);
+  if (a.hidden % kPV != 0 || !aligned_to(a.table, 16) || !aligned_to(a.out, 16)) return launch_scaled_lookup_t<DT, 1, 4>(a, stream);
+  // few rows: one vector per lane spreads them over more warps
+  if (a.n_ids * (a.hidden / kPV) < static_cast<int64_t>(sm_count()) * 2048) return launch_scaled_lookup_t<DT, kPV, 1>(a, stream);
+  return launch_scaled_lookup_t<DT, kPV, 4>(a, stream);
+}
+
+// The caller's ids.
+struct Ids {
+  const void* ids;
+  int64_t n, vocab, padding_id;
+  int id_dtype;
+  cb200_status* status;
+};
+
+// Sorting key of token i: its id, or `vocab` for one that contributes nothing.
+__device__ __forceinline__ uint32_t key_of_id(const Ids& a, int64_t i, bool report) {
+  const uint64_t id = read_id(a.ids, a.id_dtype, i);
+  if (id >= static_cast<uint64_t>(a.vocab)) {
+    if (report) report_status(a.status, CB200_STATUS_INVALID_INDEX, i, static_cast<int64_t>(id), a.vocab);
+    return static_cast<uint32_t>(a.vocab);
+  }
+  return static_cast<int64_t>(id) == a.padding_id ? static_cast<uint32_t>(a.vocab) : static_cast<uint32_t>(id);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -109,13 +150,16 @@ cudaError_t launch_scaled_lookup_dt(const ScaledLookupArgs& a, cudaStream_t stre
 constexpr int kZeroRows = 8;  // rows per warp and visit; divides 32
 
 struct ZeroFill {
-  unsigned char* out;  // the table's gradient
+  unsigned char* out;    // the table's gradient
   int64_t row_bytes;
-  int64_t begin, end;  // rows that this launch looks after
-  int vectors;         // whether rows are whole, aligned 16-byte vectors
+  int vectors;           // whether rows are whole, aligned 16-byte vectors
+  unsigned char* present;  // [vocab] whether an id points at the row
+  int64_t begin, end;    // rows that this launch looks after
+  unsigned blocks;       // its first blocks, which do
 };
 
-// A warp writes zeros to the rows v0 + k of the set bits k of `rows`.
+// A warp writes zeros to the rows v0 + k of the set bits k of `rows`.  (Bulk copies out of a block of zeros in shared
+// memory are no faster for rows of 8 KB and take twice as long for rows of 2 KB.)
 __device__ __forceinline__ void fill_rows(const ZeroFill& z, int64_t v0, unsigned rows) {
   const int lane = threadIdx.x & 31;
   for (; rows != 0; rows &= rows - 1) {
@@ -129,51 +173,79 @@ __device__ __forceinline__ void fill_rows(const ZeroFill& z, int64_t v0, unsigne
   }
 }
 
+// Block `block` of the launch's first z.blocks fills its part of the rows [z.begin, z.end).
+__device__ __forceinline__ void fill_share(const ZeroFill& z, unsigned block) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  for (int64_t v0 = z.begin + (static_cast<int64_t>(block) * warps + (threadIdx.x >> 5)) * kZeroRows; v0 < z.end;
+       v0 += static_cast<int64_t>(z.blocks) * warps * kZeroRows) {
+    const int64_t v = v0 + lane;
+    const bool empty = lane < kZeroRows && v < z.end && z.present[v] == 0;
+    fill_rows(z, v0, __ballot_sync(0xFFFFFFFFu, empty));
+  }
+}
+
+// The same without `present`, for few tokens: the block takes an equal share of the table's rows, marks in shared memory
+// which of them the ids name, and writes zeros to the rest.
+constexpr int kMarkWords = 2048;  // rows marked at a time: 32 per word
+
+__device__ __noinline__ void mark_and_fill(const ZeroFill& z, const Ids& t, unsigned block, void* shared) {
+  uint32_t* words = static_cast<uint32_t*>(shared);
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = static_cast<int>(t.n);
+  const int64_t begin = t.vocab * block / z.blocks, end = t.vocab * (block + 1) / z.blocks;
+  for (int64_t from = begin; from < end; from += kMarkWords * 32) {
+    const int64_t to = from + kMarkWords * 32 < end ? from + kMarkWords * 32 : end;
+    const int rows = static_cast<int>(to - from);
+    for (int w = threadIdx.x; w < (rows + 31) / 32; w += blockDim.x) words[w] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int64_t key = key_of_id(t, i, false);
+      if (key >= from && key < to) atomicOr(&words[(key - from) >> 5], 1u << ((key - from) & 31));
+    }
+    __syncthreads();
+    for (int r = warp * kZeroRows; r < rows; r += warps * kZeroRows) {
+      const unsigned inside = rows - r < kZeroRows ? (1u << (rows - r)) - 1u : (1u << kZeroRows) - 1u;
+      fill_rows(z, from + r, ~(words[r >> 5] >> (r & 31)) & inside);
+    }
+    __syncthreads();
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (id, position), digits of at most 9 bits.  Tokens that contribute nothing (bad ids, padding)
-// get the key `vocab` and end up behind all rows.
-//   up to 4096 tokens: one CTA does every digit in shared memory;
-//   more: one launch counts the first digit per CTA, then one launch per digit moves the keys: every CTA derives
-//   from all the counts where its keys of each digit go, and counts the next digit for the CTA that will read them.
-// A CTA takes a contiguous span of keys in tiles of 2048.
+// Stable sort of (id, position).  Tokens that contribute nothing (bad ids, padding) get the key `vocab` and end up behind
+// all rows.
+//   up to 8192 tokens: one launch; a token's place is the number of tokens that sort before it, counted over all of
+//   them by a CTA per 32 tokens (67 M comparisons at most, a few microseconds on the whole GPU);
+//   more: radix sort, digits of at most 9 bits.  One launch counts the first digit per CTA, then one launch per digit
+//   moves the keys: every CTA derives from all the counts where its keys of each digit go, and counts the next digit
+//   for the CTA that will read them.  A CTA takes a contiguous span of keys in tiles of 2048.
 // ---------------------------------------------------------------------------------------------
 constexpr int kSortItems = 4;
 constexpr int kSortThreads = 512;
 constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kSmallThreads = 1024;
-constexpr int kSmallMax = kSmallThreads * kSortItems;
+constexpr int kRankThreads = 256;
+constexpr int kRankWarps = kRankThreads / 32;
+constexpr int kRankMax = 8192;
 constexpr int kSortMaxBits = 9;
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 constexpr int kSortMaxCtas = 512;
 
 struct SortArgs {
-  const void* ids;           // first digit: the caller's ids
+  Ids tokens;                // first digit: the keys come from here
   const uint32_t* keys_in;   // later digits
   const uint32_t* values_in;
   uint32_t* keys_out;
   uint32_t* values_out;
   uint32_t* counts;          // [ctas][bins] of this digit
   uint32_t* next_counts;     // of the next one; NULL at the last
-  uint32_t* long_runs;       // their number is cleared by the sort's first launch
-  unsigned char* present;    // fresh gradient: [vocab] zeros, set to 1 by the count launch where an id points
-  ZeroFill zero;             // what the launch's blocks behind the sorting ones fill
-  unsigned sort_blocks;
-  int64_t n, vocab, padding_id;
-  int id_dtype;
-  cb200_status* status;
+  uint32_t* n_long;          // number of long runs: cleared by the sort's first launch
+  ZeroFill zero;
+  unsigned sort_blocks;      // behind the zero-filling blocks
+  int64_t n;
   int64_t span;              // keys per CTA, a multiple of kSortTile
-  int shift, width, passes;  // digit position and bits; digits in all
+  int shift, width;          // digit position and bits
   int first;
 };
-
-__device__ __forceinline__ uint32_t key_of_id(const SortArgs& a, int64_t i, bool report) {
-  const uint64_t id = read_id(a.ids, a.id_dtype, i);
-  if (id >= static_cast<uint64_t>(a.vocab)) {
-    if (report) report_status(a.status, CB200_STATUS_INVALID_INDEX, i, static_cast<int64_t>(id), a.vocab);
-    return static_cast<uint32_t>(a.vocab);
-  }
-  return static_cast<int64_t>(id) == a.padding_id ? static_cast<uint32_t>(a.vocab) : static_cast<uint32_t>(id);
-}
 
 // Exclusive sum over the CTA's threads; `totals` holds one word per warp.
 __device__ __forceinline__ uint32_t exclusive_scan(uint32_t own, uint32_t* totals) {
@@ -219,16 +291,22 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[kSortItems], 
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t hist[kSortMaxBins];
+  __shared__ uint32_t marked[kSortThreads];  // some id of each residue that was marked already, or none
   const int bins = 1 << a.width;
   if (threadIdx.x < bins) hist[threadIdx.x] = 0;
+  marked[threadIdx.x] = 0xFFFFFFFFu;
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.long_runs[0] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_long = 0;
   const int64_t begin = blockIdx.x * a.span;
   const int64_t end = begin + a.span < a.n ? begin + a.span : a.n;
   for (int64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
-    const uint32_t key = key_of_id(a, i, true);
+    const uint32_t key = key_of_id(a.tokens, i, true);
     atomicAdd(&hist[key & (bins - 1)], 1u);
-    if (a.present != nullptr && key < a.vocab) a.present[key] = 1;
+    // thousands of stores to a hot id's byte would queue up in one place
+    if (a.zero.present != nullptr && key < a.tokens.vocab && marked[key % kSortThreads] != key) {
+      marked[key % kSortThreads] = key;
+      a.zero.present[key] = 1;
+    }
   }
   __syncthreads();
   if (threadIdx.x < bins) {
@@ -237,22 +315,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs
   }
 }
 
-// Blocks [0, sort_blocks) move the keys of one digit; the others fill rows without tokens meanwhile, which the sort
-// leaves the memory free for.
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs a) {
-  if (blockIdx.x >= a.sort_blocks) {
-    const int64_t warps = static_cast<int64_t>(gridDim.x - a.sort_blocks) * (kSortThreads / 32);
-    for (int64_t v0 = a.zero.begin + (static_cast<int64_t>(blockIdx.x - a.sort_blocks) * (kSortThreads / 32) + (threadIdx.x >> 5)) * kZeroRows;
-         v0 < a.zero.end; v0 += warps * kZeroRows) {
-      const int64_t v = v0 + (threadIdx.x & 31);
-      const bool empty = (threadIdx.x & 31) < kZeroRows && v < a.zero.end && a.present[v] == 0;
-      fill_rows(a.zero, v0, __ballot_sync(0xFFFFFFFFu, empty));
-    }
-    return;
-  }
   __shared__ uint32_t base[kSortMaxBins];
   __shared__ uint32_t totals[kSortThreads / 32];
   __shared__ uint16_t count[kSortThreads / 32][kSortMaxBins];
+  if (blockIdx.x < a.zero.blocks) return fill_share(a.zero, blockIdx.x);
+  const unsigned block = blockIdx.x - a.zero.blocks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << a.width;
 
   // first slot of this CTA's keys of digit d: all smaller digits, and this digit in the CTAs before
@@ -261,14 +329,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs 
 #pragma unroll 16
     for (unsigned t = 0; t < a.sort_blocks; ++t) {
       const uint32_t c = a.counts[static_cast<int64_t>(t) * bins + threadIdx.x];
-      before += t < blockIdx.x ? c : 0u;
+      before += t < block ? c : 0u;
       total += c;
     }
   }
   before += exclusive_scan(total, totals);
   base[threadIdx.x] = before;
 
-  const int64_t begin = blockIdx.x * a.span;
+  const int64_t begin = block * a.span;
   const int64_t end = begin + a.span < a.n ? begin + a.span : a.n;
   for (int64_t tile = begin; tile < end; tile += kSortTile) {
     uint32_t* zero = reinterpret_cast<uint32_t*>(&count[0][0]);
@@ -281,7 +349,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs 
     for (int j = 0; j < kSortItems; ++j) {
       const int64_t i = mine + j * 32;
       live[j] = i < end;
-      key[j] = !live[j] ? 0u : a.first ? key_of_id(a, i, false) : a.keys_in[i];
+      key[j] = !live[j] ? 0u : a.first ? key_of_id(a.tokens, i, false) : a.keys_in[i];
       value[j] = !live[j] ? 0u : a.first ? static_cast<uint32_t>(i) : a.values_in[i];
       digit[j] = (key[j] >> a.shift) & (bins - 1);
     }
@@ -313,88 +381,40 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs 
   }
 }
 
-// Block 0 sorts up to kSmallMax tokens.  The others fill the rows without tokens: each takes an equal share of the
-// table's rows, marks in shared memory which of them the ids name, and writes zeros to the rest.
-constexpr int kMarkWords = 4096;  // rows marked at a time: 32 per word
-constexpr int kSmallSmem = (2 * kSmallMax + kSortMaxBins + kSmallThreads / 32) * 4 + kSmallThreads / 32 * kSortMaxBins * 2;
-static_assert(kMarkWords * 4 <= kSmallSmem, "the marks fit");
-
-__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArgs a) {
-  extern __shared__ uint32_t pairs[];  // [keys | values][kSmallMax], then what the digits need
-  if (blockIdx.x > 0) {
-    const int64_t shares = gridDim.x - 1, share = blockIdx.x - 1;
-    const int64_t begin = a.vocab * share / shares, end = a.vocab * (share + 1) / shares;
-    for (int64_t from = begin; from < end; from += kMarkWords * 32) {
-      const int64_t to = from + kMarkWords * 32 < end ? from + kMarkWords * 32 : end;
-      const int words = static_cast<int>((to - from + 31) / 32);
-      for (int w = threadIdx.x; w < words; w += kSmallThreads) pairs[w] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < a.n; i += kSmallThreads) {
-        const int64_t key = key_of_id(a, i, false);
-        if (key >= from && key < to) atomicOr(&pairs[(key - from) >> 5], 1u << ((key - from) & 31));
-      }
-      __syncthreads();
-      const int rows = static_cast<int>(to - from);
-      for (int r = (threadIdx.x >> 5) * kZeroRows; r < rows; r += kSmallThreads / 32 * kZeroRows) {
-        const unsigned inside = rows - r < kZeroRows ? (1u << (rows - r)) - 1u : (1u << kZeroRows) - 1u;
-        fill_rows(a.zero, from + r, ~(pairs[r >> 5] >> (r & 31)) & inside);
-      }
-      __syncthreads();
-    }
-    return;
+// A block places 32 tokens.
+__global__ void __launch_bounds__(kRankThreads) sort_small_kernel(const SortArgs a) {
+  extern __shared__ __align__(16) uint32_t words[];
+  __shared__ uint32_t part[kRankWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = static_cast<int>(a.n);
+  const int first = static_cast<int>(blockIdx.x) * 32;  // this block's tokens
+  if (first == 0 && threadIdx.x == 0) *a.n_long = 0;
+  const int padded = (n + 31) / 32 * 32;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < padded; i += kRankThreads) words[i] = i < n ? key_of_id(a.tokens, i, false) : 0xFFFFFFFFu;
+  if (threadIdx.x < 32 && first + threadIdx.x < n) key_of_id(a.tokens, first + threadIdx.x, true);  // reports a bad one
+  __syncthreads();
+  // lane: one token; warp: every eighth group of four others.  A token before it sorts before it with an equal key.
+  const uint32_t key = words[first + lane];
+  uint32_t before = 0;
+  const uint4* fours = reinterpret_cast<const uint4*>(words);
+#pragma unroll 4
+  for (int j = warp; j < first / 4; j += kRankWarps) {
+    const uint4 k = fours[j];
+    before += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
   }
-  uint32_t* base = pairs + 2 * kSmallMax;       // [kSortMaxBins]
-  uint32_t* totals = base + kSortMaxBins;       // [warps]
-  uint16_t(*count)[kSortMaxBins] = reinterpret_cast<uint16_t(*)[kSortMaxBins]>(totals + kSmallThreads / 32);  // [warps]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << a.width, n = static_cast<int>(a.n);
-  if (threadIdx.x == 0) a.long_runs[0] = 0;
-  const int mine = warp * (32 * kSortItems) + lane;
-  uint32_t key[kSortItems], value[kSortItems], digit[kSortItems], rank[kSortItems];
-  bool live[kSortItems];
-#pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int i = mine + j * 32;
-    live[j] = i < n;
-    key[j] = live[j] ? key_of_id(a, i, true) : 0u;
-    value[j] = i;
+#pragma unroll 4
+  for (int j = first / 4 + 8 + warp; j < padded / 4; j += kRankWarps) {
+    const uint4 k = fours[j];
+    before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
   }
-  for (int p = 0; p < a.passes; ++p) {
-    uint32_t* zero = reinterpret_cast<uint32_t*>(&count[0][0]);
-#pragma unroll
-    for (int k = 0; k < kSmallThreads / 32 * kSortMaxBins / 2 / kSmallThreads; ++k) zero[k * kSmallThreads + threadIdx.x] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j) digit[j] = (key[j] >> (p * a.width)) & (bins - 1);
-    warp_ranks(digit, live, rank, count[warp], a.width);
-    __syncthreads();
-    uint32_t sum = 0;
-    if (threadIdx.x < bins) {
-#pragma unroll
-      for (int w = 0; w < kSmallThreads / 32; ++w) {
-        const uint32_t c = count[w][threadIdx.x];
-        count[w][threadIdx.x] = static_cast<uint16_t>(sum);
-        sum += c;
-      }
-    }
-    const uint32_t first = exclusive_scan(sum, totals);
-    if (threadIdx.x < kSortMaxBins) base[threadIdx.x] = first;
-    __syncthreads();
-    const bool last = p + 1 == a.passes;
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      if (!live[j]) continue;
-      const uint32_t at = base[digit[j]] + count[warp][digit[j]] + rank[j];
-      (last ? a.keys_out : pairs)[at] = key[j];
-      (last ? a.values_out : pairs + kSmallMax)[at] = value[j];
-    }
-    if (last) break;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      if (!live[j]) continue;
-      key[j] = pairs[mine + j * 32];
-      value[j] = pairs[kSmallMax + mine + j * 32];
-    }
+  if (warp == 0)
+    for (int l = 0; l < 32; ++l) before += l < lane ? words[first + l] <= key : words[first + l] < key;
+  part[warp][lane] = before;
+  __syncthreads();
+  if (warp == 0 && first + lane < n) {
+    for (int w = 1; w < kRankWarps; ++w) before += part[w][lane];
+    a.keys_out[before] = key;
+    a.values_out[before] = static_cast<uint32_t>(first + lane);
   }
 }
 
@@ -403,51 +423,31 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArg
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunk = 32;            // sorted tokens per chunk sum
 constexpr int kLongRun = 2 * kChunk;  // runs of at least this many tokens contain a whole chunk and are added by a CTA
-constexpr int kMaxGroup = 16;         // sorted positions per warp and visit, at most
+constexpr int kMaxGroup = 16;         // sorted positions per warp and visit, at most: with kLongRun - 1 behind them fewer than 96
 
 struct SumArgs {
   const void* grad;
   int64_t grad_stride;
   const uint32_t* keys;    // sorted
   const uint32_t* tokens;  // their positions
-  int2* runs;              // [vocab] first and one-past-last sorted index of a row's tokens
   float* chunk_sums;       // [n / kChunk][hidden]
-  uint32_t* long_runs;     // [0]: their number, then the ids that have one, in no particular order
+  uint32_t* n_long;        // number of long runs
+  uint2* long_runs;        // {one past its last sorted index, id} of each, in no particular order
+  uint32_t* begins;        // [vocab] where the long runs begin; nothing for other ids
   void* out;
   int64_t n, vocab;
   int hidden;
   float scale;
   int units;               // VEC-element units per row
-  int chunk_tiles, tiles;  // tiles of units per row: of 32 for chunks and long runs, of 32 * kRowVecs for the others
+  int tiles;               // tiles of 32 units per row
   int group;               // sorted positions per warp and visit
-  unsigned long_blocks;    // of row_sums_kernel, for the long runs
+  unsigned long_blocks;    // the first blocks, for the long runs
+  ZeroFill zero;           // few tokens: the next blocks fill the rows without tokens
+  Ids ids;                 // which they look for in the ids
 };
-#ifndef RV
-#define RV 1
-#endif
-#ifndef RB
-#define RB 4
-#endif
-constexpr int kRowVecs = RV;    // units per lane of a row tile
-constexpr int kRowBatch = RB;   // tokens whose loads are in flight together
 constexpr int kChunkBatch = 8;
+constexpr int kTokenBatch = 8;
 
-// One VEC-element unit as it lies in memory.
-template <int DT, int VEC>
-struct Unit {
-  uint4 v;
-};
-template <int DT>
-struct Unit<DT, 1> {
-  float v;
-};
-template <int DT, int VEC>
-__device__ __forceinline__ Unit<DT, VEC> load_unit(const void* base, int64_t elem) {
-  Unit<DT, VEC> u;
-  if constexpr (VEC == 1) u.v = load_elem<DT>(base, elem);
-  else u.v = ldg_stream(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + elem * Elem<DT>::kBytes));
-  return u;
-}
 template <int DT, int VEC>
 __device__ __forceinline__ void add_unit(const Unit<DT, VEC>& u, float (&acc)[VEC]) {
   if constexpr (VEC == 1) {
@@ -460,24 +460,6 @@ __device__ __forceinline__ void add_unit(const Unit<DT, VEC>& u, float (&acc)[VE
   }
 }
 
-// acc += grad rows of the tokens s, s + step, ... below e, in that order, for unit u of the row.
-template <int DT, int VEC>
-__device__ __forceinline__ void add_tokens(const SumArgs& a, int u, int64_t s, int64_t e, int64_t step, float (&acc)[VEC]) {
-  for (; s < e; s += step * kChunkBatch) {
-    Unit<DT, VEC> q[kChunkBatch];
-    const int64_t left = (e - s + step - 1) / step;
-    uint32_t token[kChunkBatch];
-#pragma unroll
-    for (int k = 0; k < kChunkBatch; ++k) token[k] = a.tokens[k < left ? s + k * step : s];
-#pragma unroll
-    for (int k = 0; k < kChunkBatch; ++k)
-      if (k < left) q[k] = load_unit<DT, VEC>(a.grad, static_cast<int64_t>(token[k]) * a.grad_stride + static_cast<int64_t>(u) * VEC);
-#pragma unroll
-    for (int k = 0; k < kChunkBatch; ++k)
-      if (k < left) add_unit<DT, VEC>(q[k], acc);
-  }
-}
-
 // Unit u of a table row from its sum; `old` is what it holds, read only with ACC.
 template <int DTO, int VEC, bool ACC>
 __device__ __forceinline__ void write_unit(const SumArgs& a, int64_t row, int u, const float (&acc)[VEC], const float (&old)[VEC]) {
@@ -487,45 +469,85 @@ __device__ __forceinline__ void write_unit(const SumArgs& a, int64_t row, int u,
   store_floats<DTO, VEC>(a.out, row * a.hidden + static_cast<int64_t>(u) * VEC, f);
 }
 
-// Marks where the run of every id begins and ends, and adds up the chunks that one id fills.
+// Lists the long runs and adds up the chunks that one id fills.
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256) chunk_sums_kernel(const SumArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (int64_t i = me; i < a.n; i += threads) {
+  for (int64_t i = me; i + kLongRun <= a.n; i += threads) {
     const uint32_t key = a.keys[i];
-    if (key >= a.vocab) continue;
-    if (i == 0 || a.keys[i - 1] != key) {
-      a.runs[key].x = static_cast<int>(i);
-      if (i + kLongRun <= a.n && a.keys[i + kLongRun - 1] == key) a.long_runs[1 + atomicAdd(a.long_runs, 1u)] = key;
-    }
-    if (i + 1 == a.n || a.keys[i + 1] != key) a.runs[key].y = static_cast<int>(i + 1);
+    if (key >= a.vocab || a.keys[i + kLongRun - 1] != key) continue;
+    if (i == 0 || a.keys[i - 1] != key) a.begins[key] = static_cast<uint32_t>(i);
+    const int64_t behind = i + kLongRun;  // of the 64 positions from i on
+    if (behind == a.n || a.keys[behind] != key) a.long_runs[atomicAdd(a.n_long, 1u)] = make_uint2(static_cast<uint32_t>(behind), key);
   }
-  const int64_t n_items = a.n / kChunk * a.chunk_tiles;
+  const int64_t n_items = a.n / kChunk * a.tiles;
   for (int64_t item = me >> 5; item < n_items; item += threads >> 5) {
-    const int64_t c = item / a.chunk_tiles;
-    const uint32_t key = a.keys[c * kChunk];
-    if (key >= a.vocab || a.keys[c * kChunk + kChunk - 1] != key) continue;
-    const int u = static_cast<int>(item - c * a.chunk_tiles) * 32 + lane;
-    if (u >= a.units) continue;
+    const int64_t c = item / a.tiles;
+    const uint32_t key = a.keys[c * kChunk + lane % kChunk], token = a.tokens[c * kChunk + lane % kChunk];
+    if (key >= a.vocab || !__all_sync(0xFFFFFFFFu, key == __shfl_sync(0xFFFFFFFFu, key, 0))) continue;
+    const int u = static_cast<int>(item - c * a.tiles) * 32 + lane;
     float acc[VEC] = {};
-    add_tokens<DT, VEC>(a, u, c * kChunk, (c + 1) * kChunk, 1, acc);
-    store_floats<kDtF32, VEC>(a.chunk_sums, c * a.hidden + static_cast<int64_t>(u) * VEC, acc);
+#pragma unroll
+    for (int t0 = 0; t0 < kChunk; t0 += kChunkBatch) {
+      Unit<DT, VEC> q[kChunkBatch];
+#pragma unroll
+      for (int t = 0; t < kChunkBatch; ++t) {
+        const int64_t at = static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, token, t0 + t)) * a.grad_stride;
+        if (u < a.units) q[t] = load_unit<DT, VEC>(a.grad, at + static_cast<int64_t>(u) * VEC);
+      }
+#pragma unroll
+      for (int t = 0; t < kChunkBatch; ++t)
+        if (u < a.units) add_unit<DT, VEC>(q[t], acc);
+    }
+    if (u < a.units) store_floats<kDtF32, VEC>(a.chunk_sums, c * a.hidden + static_cast<int64_t>(u) * VEC, acc);
   }
 }
 
-// A long run, by a CTA per tile of 32 units: its whole chunks and the tokens before and behind them, each warp every
-// eighth, then the warps' parts in order.
+// One past the last sorted index of the run that holds index `at`: the keys behind it are searched 32 ways at a time.
+__device__ __forceinline__ int64_t run_end(const SumArgs& a, int64_t at) {
+  const uint32_t key = a.keys[at];
+  const int lane = threadIdx.x & 31;
+  int64_t lo = at, hi = a.n;  // keys[lo] == key; hi: behind the run, or the end
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t probe = lo + (lane + 1) * step;
+    const unsigned in = __ballot_sync(0xFFFFFFFFu, probe < hi && a.keys[probe < hi ? probe : at] == key);
+    const int inside = __popc(in);  // the probes are in order: the first `inside` of them are in the run
+    if (lo + (inside + 1) * step < hi) hi = lo + (inside + 1) * step;
+    lo += inside * step;
+  }
+  return hi;
+}
+
+// A long run [begin, end) of id `key`, by a CTA per tile of 32 units: the tokens before and behind its whole chunks (all
+// of them where there are no chunk sums) and the chunk sums, each warp every eighth, then the warps' parts in order.
 template <int DT, int DTO, int VEC, bool ACC>
-__device__ __noinline__ void add_long_run(const SumArgs& a, uint32_t key, int tile, float (*part)[32 * VEC]) {
+__device__ __noinline__ void add_long_run(const SumArgs& a, int64_t begin, int64_t end, uint32_t key, int tile, float (*part)[32 * VEC]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int2 run = a.runs[key];
   const int u = tile * 32 + lane;
-  const int64_t first = (run.x + kChunk - 1) / kChunk, last = run.y / kChunk;  // chunks [first, last) are whole
+  const int64_t first = a.chunk_sums == nullptr ? 0 : (begin + kChunk - 1) / kChunk, last = a.chunk_sums == nullptr ? 0 : end / kChunk;
+  // tokens outside the chunks [first, last): index e < head is begin + e, the others go on at the last chunk's end
+  const int64_t head = first == last ? end - begin : first * kChunk - begin, loose = first == last ? head : head + end - last * kChunk;
   float acc[VEC] = {};
+  for (int64_t e = warp; e < loose; e += 8 * kTokenBatch) {
+    uint32_t token[kTokenBatch];
+    Unit<DT, VEC> q[kTokenBatch];
+#pragma unroll
+    for (int k = 0; k < kTokenBatch; ++k) {
+      const int64_t i = e + 8 * k < loose ? e + 8 * k : e;
+      token[k] = a.tokens[i < head ? begin + i : last * kChunk + (i - head)];
+    }
+#pragma unroll
+    for (int k = 0; k < kTokenBatch; ++k)
+      if (e + 8 * k < loose && u < a.units)
+        q[k] = load_unit<DT, VEC>(a.grad, static_cast<int64_t>(token[k]) * a.grad_stride + static_cast<int64_t>(u) * VEC);
+#pragma unroll
+    for (int k = 0; k < kTokenBatch; ++k)
+      if (e + 8 * k < loose && u < a.units) add_unit<DT, VEC>(q[k], acc);
+  }
   if (u < a.units) {
-    add_tokens<DT, VEC>(a, u, run.x + warp, first * kChunk, 8, acc);
     for (int64_t p = first + warp; p < last; p += 8 * 4) {
       float f[4][VEC];
 #pragma unroll
@@ -538,7 +560,6 @@ __device__ __noinline__ void add_long_run(const SumArgs& a, uint32_t key, int ti
 #pragma unroll
           for (int i = 0; i < VEC; ++i) acc[i] += f[k][i];
     }
-    add_tokens<DT, VEC>(a, u, last * kChunk + warp, run.y, 8, acc);
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) part[warp][i * 32 + lane] = acc[i];
@@ -554,96 +575,232 @@ __device__ __noinline__ void add_long_run(const SumArgs& a, uint32_t key, int ti
   __syncthreads();
 }
 
-// Blocks [0, long_blocks): the long runs.  The others: a warp takes `group` sorted positions and a tile of columns
-// and adds the runs that begin there -- one contiguous stretch of the sorted list (but for long runs), gone through
-// in batches whose loads are in flight together, whatever the runs' lengths.
-#ifndef TB
-#define TB 4
-#endif
-#ifndef RMB
-#define RMB 3
-#endif
+// The runs that begin in a group of sorted positions show in the keys of the positions themselves and of the 63 behind
+// them: a window of 96 keys, three per lane.
+struct Window {
+  uint32_t key[3], token[3];
+  uint32_t last;  // the key before the window
+  __device__ __forceinline__ void load(const SumArgs& a, int64_t at) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int64_t i = at + 32 * k + lane;
+      key[k] = i < a.n ? a.keys[i] : static_cast<uint32_t>(a.vocab);
+      token[k] = i < a.n ? a.tokens[i] : 0u;
+    }
+    last = at > 0 && at < a.n ? a.keys[at - 1] : 0xFFFFFFFFu;
+  }
+  __device__ __forceinline__ uint32_t key_at(int p) const {
+    return __shfl_sync(0xFFFFFFFFu, p < 32 ? key[0] : p < 64 ? key[1] : key[2], p & 31);
+  }
+  __device__ __forceinline__ uint32_t token_at(int p) const {
+    return __shfl_sync(0xFFFFFFFFu, p < 32 ? token[0] : p < 64 ? token[1] : token[2], p & 31);
+  }
+};
+
+// The tokens of those runs: positions [from, to) of the window, without a long run, which can only be the last one;
+// bit p of heads: a run (or what is no row) begins at position p.
+struct Stretch {
+  unsigned heads[3];
+  int from, to;
+  __device__ __forceinline__ void find(const SumArgs& a, const Window& w) {
+    const int lane = threadIdx.x & 31;
+    uint32_t last = w.last;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, w.key[k], 1);
+      heads[k] = __ballot_sync(0xFFFFFFFFu, w.key[k] != (lane == 0 ? last : up));
+      last = __shfl_sync(0xFFFFFFFFu, w.key[k], 31);
+    }
+    from = to = 0;
+    const unsigned mine = heads[0] & ((1u << a.group) - 1u) & __ballot_sync(0xFFFFFFFFu, w.key[0] < a.vocab);
+    if (mine == 0) return;
+    from = __ffs(mine) - 1;
+    const int final = 31 - __clz(mine);
+    const unsigned behind = heads[0] & ~((2u << final) - 1u);
+    const int end = behind ? __ffs(behind) - 1 : heads[1] ? 32 + __ffs(heads[1]) - 1 : heads[2] ? 64 + __ffs(heads[2]) - 1 : 96;
+    to = end - final < kLongRun ? end : final;
+  }
+  __device__ __forceinline__ bool last_of_run(int p) const {
+    const int next = p + 1;
+    return next == to || (((next < 32 ? heads[0] : next < 64 ? heads[1] : heads[2]) >> (next & 31)) & 1u);
+  }
+};
+
+// The blocks for the long runs.
 template <int DT, int DTO, int VEC, bool ACC>
-__global__ void __launch_bounds__(256, RMB) row_sums_kernel(const SumArgs a) {
-  __shared__ float part[8][32 * VEC];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x < a.long_blocks) {
-    const int64_t n_items = static_cast<int64_t>(a.long_runs[0]) * a.chunk_tiles;
-    for (int64_t item = blockIdx.x; item < n_items; item += a.long_blocks)
-      add_long_run<DT, DTO, VEC, ACC>(a, a.long_runs[1 + item / a.chunk_tiles], static_cast<int>(item % a.chunk_tiles), part);
+__device__ __forceinline__ void long_runs(const SumArgs& a, unsigned block, float (*part)[32 * VEC]) {
+  if (a.chunk_sums != nullptr) {
+    const int64_t n_items = static_cast<int64_t>(*a.n_long) * a.tiles;
+    for (int64_t item = block; item < n_items; item += a.long_blocks) {
+      const uint2 run = a.long_runs[item / a.tiles];
+      add_long_run<DT, DTO, VEC, ACC>(a, a.begins[run.y], run.x, run.y, static_cast<int>(item % a.tiles), part);
+    }
     return;
   }
+  // no list: a long run holds a multiple of kLongRun, and the block of the first one takes it
+  const int lane = threadIdx.x & 31;
+  const int64_t at = block / a.tiles * kLongRun;
+  const uint32_t key = a.keys[at];
+  if (key >= a.vocab || (at > 0 && a.keys[at - kLongRun] == key)) return;
+  int64_t begin = at;  // back to where the run begins, at most 63 positions
+  for (int k = 0; k < 2; ++k) {
+    const int64_t p = at - 1 - 32 * k - lane;
+    const unsigned other = ~__ballot_sync(0xFFFFFFFFu, p >= 0 && a.keys[p >= 0 ? p : 0] == key);
+    begin = at - 32 * k - (other ? __ffs(other) - 1 : 32);
+    if (other) break;
+  }
+  if (begin + kLongRun <= a.n && a.keys[begin + kLongRun - 1] == key)
+    add_long_run<DT, DTO, VEC, ACC>(a, begin, run_end(a, begin), key, static_cast<int>(block % a.tiles), part);
+}
+
+// The first long_blocks blocks: the long runs; the next zero.blocks: the rows without tokens.  The others: a warp takes `group` sorted positions and a
+// tile of 32 V vectors and adds the runs that begin there, then the next such item: one stream of tokens, whatever
+// the runs' lengths and the items' borders.  Each lane brings its V vectors of the next 15 / V tokens (7 / V with ACC) into its own
+// slots of shared memory by asynchronous copies and reads back only what it copied itself, so nothing but the copies' own
+// completion is waited for.  With ACC the warp also brings what the table holds, for a run's last token.
+template <bool ACC, int V>
+struct Ring {
+  static constexpr int kDepth = (ACC ? 8 : 16) / V;
+};
+template <int DT, int DTO, bool ACC, int V>
+__global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __grid_constant__ SumArgs a) {
+  constexpr int VEC = Elem<DT>::kPerVec, kOld = ACC ? VEC * Elem<DTO>::kBytes / 16 : 0, kSlot = V * (1 + kOld);  // 16-byte words
+  extern __shared__ __align__(16) unsigned char shared[];
+  unsigned block = blockIdx.x;
+  if (block < a.long_blocks) return long_runs<DT, DTO, VEC, ACC>(a, block, reinterpret_cast<float(*)[32 * VEC]>(shared));
+  block -= a.long_blocks;
+  if (block < a.zero.blocks) return mark_and_fill(a.zero, a.ids, block, shared);
+  block -= a.zero.blocks;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4* ring = reinterpret_cast<uint4*>(shared) + warp * (Ring<ACC, V>::kDepth * kSlot * 32) + lane;  // [slot][word][lane]
+  const int row_tiles = (a.units + 32 * V - 1) / (32 * V);
+  const int64_t n_items = (a.n + a.group - 1) / a.group * row_tiles;
+  const int64_t stride = static_cast<int64_t>(gridDim.x - a.zero.blocks - a.long_blocks) * 8;
+
+  int64_t item = static_cast<int64_t>(block) * 8 + warp;  // the next one to be opened; its window is on the way
+  Window ahead, now;
+  Stretch s;
+  s.from = s.to = 0;
+  int p = 0, tile = 0;
+  ahead.load(a, item / row_tiles * a.group);
+  uint32_t slot_row = 0, slot_end = 0, slot_tile = 0;  // lane k: of the token in slot k
+  unsigned issued = 0, done = 0;
+
+  auto issue = [&]() {
+    while (p == s.to && item < n_items) {
+      now = ahead;
+      tile = static_cast<int>(item % row_tiles);
+      item += stride;
+      ahead.load(a, item < n_items ? item / row_tiles * a.group : a.n);
+      s.find(a, now);
+      p = s.from;
+    }
+    if (p < s.to) {
+      const uint32_t row = now.key_at(p), token = now.token_at(p);
+      const bool end = s.last_of_run(p);
+      const int slot = issued % Ring<ACC, V>::kDepth, u0 = tile * (32 * V) + lane;
+      uint4* to = ring + slot * kSlot * 32;
+      const unsigned char* from = static_cast<const unsigned char*>(a.grad) + (static_cast<int64_t>(token) * a.grad_stride + static_cast<int64_t>(u0) * VEC) * Elem<DT>::kBytes;
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (u0 + 32 * k < a.units) cp_async16(to + k * 32, from + k * 512);
+      if (ACC && end) {  // 16-byte words in the order of memory, not of the lanes that will use them
+        const int u = tile * (32 * V);
+        const unsigned char* old = static_cast<const unsigned char*>(a.out) + (static_cast<int64_t>(row) * a.hidden + static_cast<int64_t>(u) * VEC) * Elem<DTO>::kBytes;
+#pragma unroll
+        for (int k = 0; k < V * kOld; ++k)
+          if (32 * k + lane < (a.units - u) * kOld) cp_async16(to + (V + k) * 32, old + (32 * k + lane) * 16);
+      }
+      if (lane == slot) {
+        slot_row = row;
+        slot_end = end;
+        slot_tile = tile;
+      }
+      ++issued;
+      ++p;
+    }
+    cp_async_commit();
+  };
+
+  float acc[V][VEC] = {};
+#pragma unroll 1
+  for (int k = 0; k < Ring<ACC, V>::kDepth - 1; ++k) issue();
+  for (;;) {
+    issue();
+    if (done == issued) break;
+    asm volatile("cp.async.wait_group %0;" ::"n"(Ring<ACC, V>::kDepth - 1) : "memory");
+    const int slot = done % Ring<ACC, V>::kDepth;
+    const uint32_t row = __shfl_sync(0xFFFFFFFFu, slot_row, slot), end = __shfl_sync(0xFFFFFFFFu, slot_end, slot);
+    const int u0 = __shfl_sync(0xFFFFFFFFu, slot_tile, slot) * (32 * V) + lane;
+    ++done;
+    const uint4* from = ring + slot * kSlot * 32;
+    if constexpr (ACC) __syncwarp();  // the other lanes' copies of what the table holds
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (u0 + 32 * k >= a.units) continue;
+      Unit<DT, VEC> q;
+      q.v = from[k * 32];
+      add_unit<DT, VEC>(q, acc[k]);
+      if (end) {
+        float old[VEC] = {};
+        if constexpr (ACC) {
+          constexpr int kPV = Elem<DTO>::kPerVec;
+#pragma unroll
+          for (int o = 0; o < kOld; ++o) {
+            float t[kPV];
+            vec_to_floats<DTO>(from[(V + k * kOld) * 32 - lane + kOld * lane + o], t);
+#pragma unroll
+            for (int i = 0; i < kPV; ++i) old[o * kPV + i] = t[i];
+          }
+        }
+        write_unit<DTO, VEC, ACC>(a, row, u0 + 32 * k, acc[k], old);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[k][i] = 0.0f;
+      }
+    }
+  }
+}
+
+// The same for rows that are not whole, aligned vectors: element by element, a few tokens' loads in flight together.
+template <int DT, int DTO, bool ACC>
+__global__ void __launch_bounds__(256) row_sums_any_kernel(const __grid_constant__ SumArgs a) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  unsigned block = blockIdx.x;
+  if (block < a.long_blocks) return long_runs<DT, DTO, 1, ACC>(a, block, reinterpret_cast<float(*)[32]>(shared));
+  block -= a.long_blocks;
+  if (block < a.zero.blocks) return mark_and_fill(a.zero, a.ids, block, shared);
+  block -= a.zero.blocks;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n_items = (a.n + a.group - 1) / a.group * a.tiles;
-  const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.long_blocks) * 8;
-  for (int64_t item = static_cast<int64_t>(blockIdx.x - a.long_blocks) * 8 + warp; item < n_items; item += n_warps) {
+  const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.zero.blocks - a.long_blocks) * 8;
+  for (int64_t item = static_cast<int64_t>(block) * 8 + warp; item < n_items; item += n_warps) {
     const int64_t group = item / a.tiles;
-    const int u0 = static_cast<int>(item - group * a.tiles) * (32 * kRowVecs) + lane;
-    // lane l < group: the row, first sorted index and number of tokens of the run that begins at position l
-    const int64_t mine = group * a.group + lane;
-    uint32_t row = 0;
-    int begin = 0, count = 0;
-    if (lane < a.group && mine < a.n) {
-      row = a.keys[mine];
-      if (row < a.vocab && (mine == 0 || a.keys[mine - 1] != row)) {
-        begin = static_cast<int>(mine);
-        count = a.runs[row].y - begin;
-        if (count >= kLongRun) count = 0;
+    const int u = static_cast<int>(item - group * a.tiles) * 32 + lane;
+    Window w;
+    Stretch s;
+    w.load(a, group * a.group);
+    s.find(a, w);
+    float acc[1] = {};
+    for (int t0 = s.from; t0 < s.to; t0 += kTokenBatch) {
+      Unit<DT, 1> q[kTokenBatch];
+#pragma unroll
+      for (int t = 0; t < kTokenBatch; ++t) {
+        const int64_t at = static_cast<int64_t>(w.token_at(t0 + t < s.to ? t0 + t : t0)) * a.grad_stride;
+        if (u < a.units) q[t] = load_unit<DT, 1>(a.grad, at + u);
       }
-    }
-    int before = count;  // tokens of the runs up to and with this lane's, then without
 #pragma unroll
-    for (int o = 1; o < kMaxGroup; o <<= 1) {
-      const int up = __shfl_up_sync(0xFFFFFFFFu, before, o);
-      if (lane >= o) before += up;
-    }
-    const int n_tokens = __shfl_sync(0xFFFFFFFFu, before, kMaxGroup - 1);
-    before -= count;
-    float acc[kRowVecs][VEC] = {};
-    for (int w = 0; w < n_tokens; w += 32) {
-      // lane l: token w + l of the stretch, and whose run it is in (the last one that starts at or before it)
-      int of = 0;
-#pragma unroll
-      for (int o = kMaxGroup / 2; o > 0; o >>= 1) {
-        const int start = __shfl_sync(0xFFFFFFFFu, before, of + o);
-        if (start <= w + lane) of += o;
-      }
-      const int starts = __shfl_sync(0xFFFFFFFFu, before, of);
-      const int from = __shfl_sync(0xFFFFFFFFu, begin, of) + (w + lane - starts);
-      const uint32_t token = w + lane < n_tokens ? a.tokens[from] : 0u;
-      const uint32_t of_row = __shfl_sync(0xFFFFFFFFu, row, of);
-      // the tokens that are their run's last
-      const unsigned ends = __ballot_sync(0xFFFFFFFFu, w + lane + 1 == starts + __shfl_sync(0xFFFFFFFFu, count, of));
-      const int here = n_tokens - w < 32 ? n_tokens - w : 32;
-      for (int t0 = 0; t0 < here; t0 += kRowBatch) {
-        Unit<DT, VEC> q[kRowBatch][kRowVecs];
-        float old[kRowBatch][kRowVecs][VEC];
-#pragma unroll
-        for (int t = 0; t < kRowBatch; ++t) {
-          const int64_t at = static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, token, (t0 + t) & 31)) * a.grad_stride;
-          const int64_t to = static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, of_row, (t0 + t) & 31)) * a.hidden;
-#pragma unroll
-          for (int k = 0; k < kRowVecs; ++k) {
-            if (t0 + t >= here || u0 + 32 * k >= a.units) continue;
-            q[t][k] = load_unit<DT, VEC>(a.grad, at + static_cast<int64_t>(u0 + 32 * k) * VEC);
-            if constexpr (ACC)
-              if ((ends >> (t0 + t)) & 1u) load_floats_plain<DTO, VEC>(a.out, to + static_cast<int64_t>(u0 + 32 * k) * VEC, old[t][k]);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < kRowBatch; ++t) {
-          const uint32_t to = __shfl_sync(0xFFFFFFFFu, of_row, (t0 + t) & 31);
-          if (t0 + t >= here) continue;
-#pragma unroll
-          for (int k = 0; k < kRowVecs; ++k) {
-            if (u0 + 32 * k >= a.units) continue;
-            add_unit<DT, VEC>(q[t][k], acc[k]);
-            if ((ends >> (t0 + t)) & 1u) {
-              write_unit<DTO, VEC, ACC>(a, to, u0 + 32 * k, acc[k], old[t][k]);
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) acc[k][i] = 0.0f;
-            }
-          }
-        }
+      for (int t = 0; t < kTokenBatch; ++t) {
+        if (t0 + t >= s.to) break;
+        const uint32_t row = w.key_at(t0 + t);
+        const bool end = s.last_of_run(t0 + t);
+        if (u >= a.units) continue;
+        add_unit<DT, 1>(q[t], acc);
+        if (!end) continue;
+        float old[1] = {};
+        if constexpr (ACC) load_floats_plain<DTO, 1>(a.out, static_cast<int64_t>(row) * a.hidden + u, old);
+        write_unit<DTO, 1, ACC>(a, row, u, acc, old);
+        acc[0] = 0.0f;
       }
     }
   }
@@ -653,8 +810,9 @@ int64_t round16(int64_t bytes) { return (bytes + 15) & ~int64_t(15); }
 
 struct Workspace {
   uint32_t *keys[2], *values[2], *counts[2];
-  int2* runs;
-  uint32_t* long_runs;
+  uint32_t* n_long;
+  uint2* long_runs;
+  uint32_t* begins;
   unsigned char* present;
   float* chunk_sums;
   int64_t bytes;
@@ -673,60 +831,66 @@ Workspace lay_out(void* base, int64_t vocab, int hidden, int64_t n) {
     w.values[i] = reinterpret_cast<uint32_t*>(take(n * 4));
     w.counts[i] = reinterpret_cast<uint32_t*>(take(int64_t(kSortMaxCtas) * kSortMaxBins * 4));
   }
-  w.runs = reinterpret_cast<int2*>(take(vocab * 8));
-  w.long_runs = reinterpret_cast<uint32_t*>(take((1 + n / kLongRun) * 4));
+  w.n_long = reinterpret_cast<uint32_t*>(take(4));
+  w.long_runs = reinterpret_cast<uint2*>(take(n / kLongRun * 8));
+  w.begins = reinterpret_cast<uint32_t*>(take(vocab * 4));
   w.present = take(vocab);
   w.chunk_sums = reinterpret_cast<float*>(take(n / kChunk * hidden * 4));
   w.bytes = at;
   return w;
 }
 
-// Sorts (id, position) into w.keys[where] / w.values[where]; without `accumulate` also fills the rows without tokens.
-cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int out_bytes, int* where, cudaStream_t stream) {
+Ids ids_of(const TableGradArgs& a) { return Ids{a.ids, a.n_ids, a.vocab, a.padding_id, a.id_dtype, a.status}; }
+
+// Takes a share of the rows that are not looked after yet, for `most` blocks of `warps` warps.
+ZeroFill share_of(ZeroFill& rest, int64_t rows, int64_t most, int warps) {
+  ZeroFill z = rest;
+  if (rest.end - rest.begin < rows) rows = rest.end - rest.begin;
+  z.end = z.begin + rows;
+  rest.begin = z.end;
+  const int64_t wanted = (rows + kZeroRows * warps - 1) / (kZeroRows * warps);
+  z.blocks = static_cast<unsigned>(wanted < most ? wanted : most);
+  return z;
+}
+
+// Sorts (id, position) into w.keys[where] / w.values[where].  `rest`: the rows in which zeros are still to be looked for
+// (none with `accumulate`).
+cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, ZeroFill& rest, cudaStream_t stream) {
   int bits = 1;
   while ((int64_t(1) << bits) <= a.vocab) ++bits;  // keys go up to vocab
   SortArgs s{};
-  s.ids = a.ids;
+  s.tokens = ids_of(a);
   s.n = a.n_ids;
-  s.vocab = a.vocab;
-  s.padding_id = a.padding_id;
-  s.id_dtype = a.id_dtype;
-  s.status = a.status;
-  s.passes = (bits + kSortMaxBits - 1) / kSortMaxBits;
-  s.width = (bits + s.passes - 1) / s.passes;
-  s.long_runs = w.long_runs;
-  s.zero.out = static_cast<unsigned char*>(a.out);
-  s.zero.row_bytes = static_cast<int64_t>(a.hidden) * out_bytes;
-  s.zero.vectors = s.zero.row_bytes % 16 == 0 && aligned_to(a.out, 16);
-  const bool zero = !a.accumulate && a.vocab > 0;
+  s.n_long = w.n_long;
   const int64_t sms = sm_count();
   *where = 0;
-  if (a.n_ids <= kSmallMax) {
-    const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(sort_small_kernel), kSmallThreads, kSmallSmem, -1, nullptr);
-    if (e != cudaSuccess) return e;
+  if (a.n_ids <= kRankMax) {
     s.keys_out = w.keys[0];
     s.values_out = w.values[0];
-    const int64_t shares = !zero ? 0 : a.vocab < 2 * sms - 1 ? a.vocab : 2 * sms - 1;
-    sort_small_kernel<<<static_cast<unsigned>(1 + shares), kSmallThreads, kSmallSmem, stream>>>(s);
+    sort_small_kernel<<<static_cast<unsigned>((a.n_ids + 31) / 32), kRankThreads, kRankMax * 4, stream>>>(s);
     return cudaGetLastError();
   }
+  const int passes = (bits + kSortMaxBits - 1) / kSortMaxBits;
+  s.width = (bits + passes - 1) / passes;
   const int64_t tiles = (a.n_ids + kSortTile - 1) / kSortTile;
   const int64_t ctas = tiles < kSortMaxCtas ? tiles : kSortMaxCtas;
   s.span = (tiles + ctas - 1) / ctas * kSortTile;
   s.sort_blocks = static_cast<unsigned>((a.n_ids + s.span - 1) / s.span);
-  if (zero) {
-    s.present = w.present;
+  if (rest.end > 0) {
     const cudaError_t e = cudaMemsetAsync(w.present, 0, static_cast<size_t>(a.vocab), stream);
     if (e != cudaSuccess) return e;
+    s.zero = rest;
+  } else {
+    s.zero.present = nullptr;
   }
-  for (int p = 0; p < s.passes; ++p) {
+  for (int p = 0; p < passes; ++p) {
     s.first = p == 0;
     s.keys_in = w.keys[(p + 1) & 1];
     s.values_in = w.values[(p + 1) & 1];
     s.keys_out = w.keys[p & 1];
     s.values_out = w.values[p & 1];
     s.counts = w.counts[p & 1];
-    s.next_counts = p + 1 < s.passes ? w.counts[(p + 1) & 1] : nullptr;
+    s.next_counts = p + 1 < passes ? w.counts[(p + 1) & 1] : nullptr;
     s.shift = p * s.width;
     if (p == 0) {
       sort_count_kernel<<<s.sort_blocks, kSortThreads, 0, stream>>>(s);
@@ -734,68 +898,98 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int out_byte
       const cudaError_t e = cudaMemsetAsync(s.next_counts, 0, static_cast<size_t>(s.sort_blocks) * 4 << s.width, stream);
       if (e != cudaSuccess) return e;
     }
-    // each digit's launch fills its share of the rows
-    s.zero.begin = a.vocab * p / s.passes;
-    s.zero.end = a.vocab * (p + 1) / s.passes;
-    const int64_t wanted = (s.zero.end - s.zero.begin + kZeroRows * kSortThreads / 32 - 1) / (kZeroRows * kSortThreads / 32);
-    const int64_t fillers = !zero ? 0 : wanted < 3 * sms ? wanted : 3 * sms;
-    sort_move_kernel<<<static_cast<unsigned>(s.sort_blocks + fillers), kSortThreads, 0, stream>>>(s);
+    s.zero = share_of(rest, p + 1 < passes ? a.vocab / passes : a.vocab, sms, kSortThreads / 32);
+    sort_move_kernel<<<s.zero.blocks + s.sort_blocks, kSortThreads, 0, stream>>>(s);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  *where = (s.passes - 1) & 1;
+  *where = (passes - 1) & 1;
   return cudaSuccess;
 }
 
 template <int DT, int DTO, int VEC, bool ACC>
-cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, cudaStream_t stream) {
+cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, ZeroFill rest, cudaStream_t stream) {
   SumArgs s{};
   s.grad = a.grad;
   s.grad_stride = a.grad_stride;
   s.keys = w.keys[where];
   s.tokens = w.values[where];
-  s.runs = w.runs;
-  s.chunk_sums = w.chunk_sums;
+  s.n_long = w.n_long;
+  s.long_runs = w.long_runs;
+  s.begins = w.begins;
   s.out = a.out;
   s.n = a.n_ids;
   s.vocab = a.vocab;
   s.hidden = a.hidden;
   s.scale = a.scale;
   s.units = a.hidden / VEC;
-  s.long_runs = w.long_runs;
-  s.chunk_tiles = (s.units + 31) / 32;
-  s.tiles = (s.units + 32 * kRowVecs - 1) / (32 * kRowVecs);
+  s.tiles = (s.units + 31) / 32;
   const int64_t sms = sm_count();
-  const int64_t chunk_items = a.n_ids / kChunk * s.chunk_tiles;
-  int64_t grid = (chunk_items > a.n_ids / 32 ? chunk_items : a.n_ids / 32) / 8 + 1;
-  if (grid > sms * 6) grid = sms * 6;
-  chunk_sums_kernel<DT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(s);
-  // fewer positions per warp where there would be too few warps to fill the GPU
-  s.group = kMaxGroup;
-  while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * s.tiles < sms * 8 * RMB * 4) s.group /= 2;
-  const int64_t items = (a.n_ids + s.group - 1) / s.group * s.tiles;
-  const int64_t max_long = a.n_ids / kLongRun * s.chunk_tiles;
-  s.long_blocks = static_cast<unsigned>(max_long < sms ? max_long : sms);
-  const int64_t token_blocks = (items + 7) / 8 < sms * TB ? (items + 7) / 8 : sms * TB;
-  row_sums_kernel<DT, DTO, VEC, ACC><<<static_cast<unsigned>(s.long_blocks + token_blocks), 256, 0, stream>>>(s);
-  return cudaGetLastError();
+  // Up to 1024 tokens a CTA adds even the longest run while the others are added (at most 16 batches of loads per warp);
+  // beyond, the launch for the chunks pays (3001 skewed tokens of 1000 columns: 58 us without, 41 with it).
+  const bool chunks = a.n_ids > 1024;
+  if (chunks) {
+    s.chunk_sums = w.chunk_sums;
+    const int64_t items = a.n_ids / kChunk * s.tiles;
+    const int64_t grid = (items + 7) / 8 < sms * 5 ? (items + 7) / 8 : sms * 5;
+    chunk_sums_kernel<DT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(s);
+  }
+  s.ids = ids_of(a);
+  s.zero = share_of(rest, rest.end - rest.begin, sms, 8);
+  const int64_t max_long = a.n_ids / kLongRun * s.tiles;
+  s.long_blocks = static_cast<unsigned>(!chunks ? (a.n_ids + kLongRun - 1) / kLongRun * s.tiles : max_long < 2 * sms ? max_long : 2 * sms);
+  const auto finish = [&](auto kern, int vectors, size_t smem) {
+    int per_sm = 4;
+    const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), 256, smem, -1, &per_sm);
+    if (e != cudaSuccess) return e;
+    // a few items per warp that is resident at once, so that the uneven runs even out; few tokens: few positions per item
+    const int64_t tiles = (s.units + 32 * vectors - 1) / (32 * vectors);
+    s.group = kMaxGroup;
+    while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * tiles < sms * per_sm * 8 * 4) s.group /= 2;
+    const int64_t items = (a.n_ids + s.group - 1) / s.group * tiles;
+    const int64_t token_blocks = (items + 7) / 8 < sms * per_sm ? (items + 7) / 8 : sms * per_sm;
+    kern<<<static_cast<unsigned>(s.zero.blocks + s.long_blocks + token_blocks), 256, smem, stream>>>(s);
+    return cudaGetLastError();
+  };
+  if constexpr (VEC > 1) {
+    // Several vectors per lane share what a token costs in instructions (1 -> 4 vectors: 120 -> 95 us for the sums of
+    // 65536 skewed tokens of 4096 columns), one keeps more tokens of a run in flight and more warps busy (3001 tokens
+    // of 1000 columns: 32 -> 18 us).
+    constexpr size_t kSmem = size_t(8) * (ACC ? 8 : 16) * 32 * (16 + (ACC ? VEC * Elem<DTO>::kBytes : 0));
+    const auto enough = [&](int vectors, int per_warp) {
+      return s.units > 16 * vectors && a.n_ids * ((s.units + 32 * vectors - 1) / (32 * vectors)) >= sms * 24 * per_warp;
+    };
+    if constexpr (!ACC)
+      if (enough(4, 16)) return finish(row_stream_kernel<DT, DTO, ACC, 4>, 4, kSmem);
+    if (enough(2, 8)) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
+    return finish(row_stream_kernel<DT, DTO, ACC, 1>, 1, kSmem);
+  } else {
+    return finish(row_sums_any_kernel<DT, DTO, ACC>, 1, kMarkWords * 4);
+  }
 }
 
 template <int DT, int DTO, int VEC>
-cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, cudaStream_t stream) {
-  return a.accumulate ? launch_sums<DT, DTO, VEC, true>(a, w, where, stream) : launch_sums<DT, DTO, VEC, false>(a, w, where, stream);
+cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, const ZeroFill& rest, cudaStream_t stream) {
+  return a.accumulate ? launch_sums<DT, DTO, VEC, true>(a, w, where, rest, stream)
+                      : launch_sums<DT, DTO, VEC, false>(a, w, where, rest, stream);
 }
 
 template <int DT, int DTO>
 cudaError_t launch_table_grad_t(const TableGradArgs& a, void* workspace, cudaStream_t stream) {
   const Workspace w = lay_out(workspace, a.vocab, a.hidden, a.n_ids);
+  ZeroFill rest{};
+  rest.out = static_cast<unsigned char*>(a.out);
+  rest.row_bytes = static_cast<int64_t>(a.hidden) * Elem<DTO>::kBytes;
+  rest.vectors = rest.row_bytes % 16 == 0 && aligned_to(a.out, 16);
+  rest.present = w.present;
+  rest.end = a.accumulate ? 0 : a.vocab;
   int where = 0;
-  const cudaError_t e = sort_tokens(a, w, Elem<DTO>::kBytes, &where, stream);
+  const cudaError_t e = sort_tokens(a, w, &where, rest, stream);
   if (e != cudaSuccess || a.vocab == 0) return e;
   constexpr int kPV = Elem<DT>::kPerVec;
   if (a.hidden % kPV == 0 && a.grad_stride % kPV == 0 && aligned_to(a.grad, 16) && aligned_to(a.out, 16))
-    return launch_sums<DT, DTO, kPV>(a, w, where, stream);
-  return launch_sums<DT, DTO, 1>(a, w, where, stream);
+    return launch_sums<DT, DTO, kPV>(a, w, where, rest, stream);
+  return launch_sums<DT, DTO, 1>(a, w, where, rest, stream);
 }
 
 }  // namespace
