@@ -8,8 +8,8 @@
 //   - row_sums_kernel writes the table rows.  Work is cut by tokens, not by rows, since a few rows of a text's table
 //     have most of its tokens: a warp adds the runs that begin at a few neighbouring sorted positions, a CTA a
 //     long run (the chunk sums and the ends that do not fill a chunk).
-// The rows without tokens are filled with zeros by further blocks of the sort's launches, which leave the memory idle, or
-// where the sort takes less than a launch's time by blocks of row_stream_kernel.
+// The rows without tokens are filled with zeros by further blocks of the launches that leave the memory idle: the radix
+// sort's, or with few tokens the chunk sums' or the row sums'.
 #include "launch.h"
 
 namespace cb200 {
@@ -145,69 +145,50 @@ __device__ __forceinline__ uint32_t key_of_id(const Ids& a, int64_t i, bool repo
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows without tokens
+// Rows without tokens.  A block fills a few neighbouring rows and ends: blocks that follow one another through memory
+// write at 7.4 TB/s, resident ones that stride over the table at 6.0 (1 GB, rows of 8 KB).
 // ---------------------------------------------------------------------------------------------
-constexpr int kZeroRows = 8;  // rows per warp and visit; divides 32
+constexpr int kFillBytes = 32 * 1024;  // per block, but at least a row
 
 struct ZeroFill {
-  unsigned char* out;    // the table's gradient
+  unsigned char* out;      // the table's gradient
   int64_t row_bytes;
-  int vectors;           // whether rows are whole, aligned 16-byte vectors
+  int vectors;             // whether rows are whole, aligned 16-byte vectors
   unsigned char* present;  // [vocab] whether an id points at the row
-  int64_t begin, end;    // rows that this launch looks after
-  unsigned blocks;       // its first blocks, which do
+  int64_t begin, end;      // rows that this launch looks after
+  int rows;                // per block
+  unsigned blocks;         // the launch's last blocks, which do
 };
 
-// A warp writes zeros to the rows v0 + k of the set bits k of `rows`.  (Bulk copies out of a block of zeros in shared
-// memory are no faster for rows of 8 KB and take twice as long for rows of 2 KB.)
-__device__ __forceinline__ void fill_rows(const ZeroFill& z, int64_t v0, unsigned rows) {
-  const int lane = threadIdx.x & 31;
-  for (; rows != 0; rows &= rows - 1) {
-    unsigned char* row = z.out + (v0 + __ffs(rows) - 1) * z.row_bytes;
-    if (z.vectors) {
+__device__ __forceinline__ void fill_rows(const ZeroFill& z, unsigned block) {
+  const int64_t first = z.begin + static_cast<int64_t>(block) * z.rows;
+  const int rows = static_cast<int>(z.end - first < z.rows ? z.end - first : z.rows);
+  unsigned char* base = z.out + first * z.row_bytes;
+  if (z.vectors) {
+    const int64_t per_row = z.row_bytes / 16;
+    if (rows == 1) {
+      if (z.present[first] != 0) return;
+      for (int64_t i = threadIdx.x; i < per_row; i += blockDim.x) stg_stream(reinterpret_cast<uint4*>(base) + i, make_uint4(0, 0, 0, 0));
+      return;
+    }
+    const unsigned row_vectors = static_cast<unsigned>(per_row);  // several rows are at most kFillBytes
 #pragma unroll 4
-      for (int64_t i = lane; i < z.row_bytes / 16; i += 32) stg_stream(reinterpret_cast<uint4*>(row) + i, make_uint4(0, 0, 0, 0));
-    } else {  // elements of 2 or 4 bytes
-      for (int64_t i = lane; i < z.row_bytes / 2; i += 32) reinterpret_cast<uint16_t*>(row)[i] = 0;
-    }
+    for (unsigned i = threadIdx.x; i < rows * row_vectors; i += blockDim.x)
+      if (z.present[first + i / row_vectors] == 0) stg_stream(reinterpret_cast<uint4*>(base) + i, make_uint4(0, 0, 0, 0));
+    return;
   }
-}
-
-// Block `block` of the launch's first z.blocks fills its part of the rows [z.begin, z.end).
-__device__ __forceinline__ void fill_share(const ZeroFill& z, unsigned block) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int64_t v0 = z.begin + (static_cast<int64_t>(block) * warps + (threadIdx.x >> 5)) * kZeroRows; v0 < z.end;
-       v0 += static_cast<int64_t>(z.blocks) * warps * kZeroRows) {
-    const int64_t v = v0 + lane;
-    const bool empty = lane < kZeroRows && v < z.end && z.present[v] == 0;
-    fill_rows(z, v0, __ballot_sync(0xFFFFFFFFu, empty));
-  }
-}
-
-// The same without `present`, for few tokens: the block takes an equal share of the table's rows, marks in shared memory
-// which of them the ids name, and writes zeros to the rest.
-constexpr int kMarkWords = 2048;  // rows marked at a time: 32 per word
-
-__device__ __noinline__ void mark_and_fill(const ZeroFill& z, const Ids& t, unsigned block, void* shared) {
-  uint32_t* words = static_cast<uint32_t*>(shared);
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = static_cast<int>(t.n);
-  const int64_t begin = t.vocab * block / z.blocks, end = t.vocab * (block + 1) / z.blocks;
-  for (int64_t from = begin; from < end; from += kMarkWords * 32) {
-    const int64_t to = from + kMarkWords * 32 < end ? from + kMarkWords * 32 : end;
-    const int rows = static_cast<int>(to - from);
-    for (int w = threadIdx.x; w < (rows + 31) / 32; w += blockDim.x) words[w] = 0;
-    __syncthreads();
-#pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int64_t key = key_of_id(t, i, false);
-      if (key >= from && key < to) atomicOr(&words[(key - from) >> 5], 1u << ((key - from) & 31));
-    }
-    __syncthreads();
-    for (int r = warp * kZeroRows; r < rows; r += warps * kZeroRows) {
-      const unsigned inside = rows - r < kZeroRows ? (1u << (rows - r)) - 1u : (1u << kZeroRows) - 1u;
-      fill_rows(z, from + r, ~(words[r >> 5] >> (r & 31)) & inside);
-    }
-    __syncthreads();
+  // a warp per row: vectors where it is aligned, elements of two bytes before and behind
+  const int lane = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
+    if (z.present[first + r] != 0) continue;
+    uint16_t* from = reinterpret_cast<uint16_t*>(base + r * z.row_bytes);
+    uint16_t* to = reinterpret_cast<uint16_t*>(base + (r + 1) * z.row_bytes);
+    uint16_t* middle = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(from) + 15) & ~uintptr_t(15));
+    uint16_t* behind = reinterpret_cast<uint16_t*>(reinterpret_cast<uintptr_t>(to) & ~uintptr_t(15));
+    if (middle >= behind) middle = behind = to;  // shorter than two vectors: element by element
+    for (uint16_t* p = from + lane; p < middle; p += 32) *p = 0;
+    for (uint16_t* p = middle + 8 * lane; p < behind; p += 8 * 32) stg_stream(reinterpret_cast<uint4*>(p), make_uint4(0, 0, 0, 0));
+    for (uint16_t* p = behind + lane; p < to; p += 32) *p = 0;
   }
 }
 
@@ -240,7 +221,7 @@ struct SortArgs {
   uint32_t* next_counts;     // of the next one; NULL at the last
   uint32_t* n_long;          // number of long runs: cleared by the sort's first launch
   ZeroFill zero;
-  unsigned sort_blocks;      // behind the zero-filling blocks
+  unsigned sort_blocks;      // before the zero-filling ones
   int64_t n;
   int64_t span;              // keys per CTA, a multiple of kSortTile
   int shift, width;          // digit position and bits
@@ -319,8 +300,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs 
   __shared__ uint32_t base[kSortMaxBins];
   __shared__ uint32_t totals[kSortThreads / 32];
   __shared__ uint16_t count[kSortThreads / 32][kSortMaxBins];
-  if (blockIdx.x < a.zero.blocks) return fill_share(a.zero, blockIdx.x);
-  const unsigned block = blockIdx.x - a.zero.blocks;
+  if (blockIdx.x >= a.sort_blocks) return fill_rows(a.zero, blockIdx.x - a.sort_blocks);
+  const unsigned block = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << a.width;
 
   // first slot of this CTA's keys of digit d: all smaller digits, and this digit in the CTAs before
@@ -391,7 +372,10 @@ __global__ void __launch_bounds__(kRankThreads) sort_small_kernel(const SortArgs
   const int padded = (n + 31) / 32 * 32;
 #pragma unroll 8
   for (int i = threadIdx.x; i < padded; i += kRankThreads) words[i] = i < n ? key_of_id(a.tokens, i, false) : 0xFFFFFFFFu;
-  if (threadIdx.x < 32 && first + threadIdx.x < n) key_of_id(a.tokens, first + threadIdx.x, true);  // reports a bad one
+  if (threadIdx.x < 32 && first + threadIdx.x < n) {
+    const uint32_t own = key_of_id(a.tokens, first + threadIdx.x, true);
+    if (a.zero.present != nullptr && own < a.tokens.vocab) a.zero.present[own] = 1;
+  }
   __syncthreads();
   // lane: one token; warp: every eighth group of four others.  A token before it sorts before it with an equal key.
   const uint32_t key = words[first + lane];
@@ -442,8 +426,7 @@ struct SumArgs {
   int tiles;               // tiles of 32 units per row
   int group;               // sorted positions per warp and visit
   unsigned long_blocks;    // the first blocks, for the long runs
-  ZeroFill zero;           // few tokens: the next blocks fill the rows without tokens
-  Ids ids;                 // which they look for in the ids
+  ZeroFill zero;
 };
 constexpr int kChunkBatch = 8;
 constexpr int kTokenBatch = 8;
@@ -471,9 +454,11 @@ __device__ __forceinline__ void write_unit(const SumArgs& a, int64_t row, int u,
 
 // Lists the long runs and adds up the chunks that one id fills.
 template <int DT, int VEC>
-__global__ void __launch_bounds__(256) chunk_sums_kernel(const SumArgs a) {
+__global__ void __launch_bounds__(256) chunk_sums_kernel(const __grid_constant__ SumArgs a) {
+  const unsigned blocks = gridDim.x - a.zero.blocks;
+  if (blockIdx.x >= blocks) return fill_rows(a.zero, blockIdx.x - blocks);
   const int lane = threadIdx.x & 31;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t threads = static_cast<int64_t>(blocks) * blockDim.x;
   const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   for (int64_t i = me; i + kLongRun <= a.n; i += threads) {
     const uint32_t key = a.keys[i];
@@ -654,11 +639,26 @@ __device__ __forceinline__ void long_runs(const SumArgs& a, unsigned block, floa
     add_long_run<DT, DTO, VEC, ACC>(a, begin, run_end(a, begin), key, static_cast<int>(block % a.tiles), part);
 }
 
-// The first long_blocks blocks: the long runs; the next zero.blocks: the rows without tokens.  The others: a warp takes `group` sorted positions and a
+// The first long_blocks blocks: the long runs; zero.blocks of the others: rows without tokens.  In the rest a warp takes `group` sorted positions and a
 // tile of 32 V vectors and adds the runs that begin there, then the next such item: one stream of tokens, whatever
 // the runs' lengths and the items' borders.  Each lane brings its V vectors of the next 15 / V tokens (7 / V with ACC) into its own
 // slots of shared memory by asynchronous copies and reads back only what it copied itself, so nothing but the copies' own
 // completion is waited for.  With ACC the warp also brings what the table holds, for a run's last token.
+// The blocks behind those for the long runs: the ones that sum and the zero-filling ones take turns, as far as there are
+// both, so that they share the SMs.  Whether this is a zero-filling one; `block` becomes its index among its kind.
+__device__ __forceinline__ bool take_turns(const SumArgs& a, unsigned& block) {
+  const unsigned sums = gridDim.x - a.long_blocks - a.zero.blocks, both = sums < a.zero.blocks ? sums : a.zero.blocks;
+  bool fill;
+  if (block < 2 * both) {
+    fill = block & 1u;
+    block >>= 1;
+  } else {
+    fill = both == sums;
+    block -= both;
+  }
+  return fill;
+}
+
 template <bool ACC, int V>
 struct Ring {
   static constexpr int kDepth = (ACC ? 8 : 16) / V;
@@ -670,8 +670,7 @@ __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __gr
   unsigned block = blockIdx.x;
   if (block < a.long_blocks) return long_runs<DT, DTO, VEC, ACC>(a, block, reinterpret_cast<float(*)[32 * VEC]>(shared));
   block -= a.long_blocks;
-  if (block < a.zero.blocks) return mark_and_fill(a.zero, a.ids, block, shared);
-  block -= a.zero.blocks;
+  if (take_turns(a, block)) return fill_rows(a.zero, block);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* ring = reinterpret_cast<uint4*>(shared) + warp * (Ring<ACC, V>::kDepth * kSlot * 32) + lane;  // [slot][word][lane]
   const int row_tiles = (a.units + 32 * V - 1) / (32 * V);
@@ -769,8 +768,7 @@ __global__ void __launch_bounds__(256) row_sums_any_kernel(const __grid_constant
   unsigned block = blockIdx.x;
   if (block < a.long_blocks) return long_runs<DT, DTO, 1, ACC>(a, block, reinterpret_cast<float(*)[32]>(shared));
   block -= a.long_blocks;
-  if (block < a.zero.blocks) return mark_and_fill(a.zero, a.ids, block, shared);
-  block -= a.zero.blocks;
+  if (take_turns(a, block)) return fill_rows(a.zero, block);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n_items = (a.n + a.group - 1) / a.group * a.tiles;
   const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.zero.blocks - a.long_blocks) * 8;
@@ -840,16 +838,15 @@ Workspace lay_out(void* base, int64_t vocab, int hidden, int64_t n) {
   return w;
 }
 
-Ids ids_of(const TableGradArgs& a) { return Ids{a.ids, a.n_ids, a.vocab, a.padding_id, a.id_dtype, a.status}; }
-
-// Takes a share of the rows that are not looked after yet, for `most` blocks of `warps` warps.
-ZeroFill share_of(ZeroFill& rest, int64_t rows, int64_t most, int warps) {
+// The next `rows` of the rows that are not looked after yet.
+ZeroFill share_of(ZeroFill& rest, int64_t rows) {
   ZeroFill z = rest;
   if (rest.end - rest.begin < rows) rows = rest.end - rest.begin;
   z.end = z.begin + rows;
   rest.begin = z.end;
-  const int64_t wanted = (rows + kZeroRows * warps - 1) / (kZeroRows * warps);
-  z.blocks = static_cast<unsigned>(wanted < most ? wanted : most);
+  // whole blocks of neighbouring rows; a grid has room for 2^31 of them
+  z.rows = static_cast<int>(z.row_bytes < kFillBytes ? kFillBytes / z.row_bytes : 1);
+  z.blocks = static_cast<unsigned>((rows + z.rows - 1) / z.rows);
   return z;
 }
 
@@ -859,10 +856,14 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, 
   int bits = 1;
   while ((int64_t(1) << bits) <= a.vocab) ++bits;  // keys go up to vocab
   SortArgs s{};
-  s.tokens = ids_of(a);
+  s.tokens = Ids{a.ids, a.n_ids, a.vocab, a.padding_id, a.id_dtype, a.status};
   s.n = a.n_ids;
   s.n_long = w.n_long;
-  const int64_t sms = sm_count();
+  if (rest.end > 0) {
+    const cudaError_t e = cudaMemsetAsync(w.present, 0, static_cast<size_t>(a.vocab), stream);
+    if (e != cudaSuccess) return e;
+    s.zero.present = w.present;
+  }
   *where = 0;
   if (a.n_ids <= kRankMax) {
     s.keys_out = w.keys[0];
@@ -876,13 +877,6 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, 
   const int64_t ctas = tiles < kSortMaxCtas ? tiles : kSortMaxCtas;
   s.span = (tiles + ctas - 1) / ctas * kSortTile;
   s.sort_blocks = static_cast<unsigned>((a.n_ids + s.span - 1) / s.span);
-  if (rest.end > 0) {
-    const cudaError_t e = cudaMemsetAsync(w.present, 0, static_cast<size_t>(a.vocab), stream);
-    if (e != cudaSuccess) return e;
-    s.zero = rest;
-  } else {
-    s.zero.present = nullptr;
-  }
   for (int p = 0; p < passes; ++p) {
     s.first = p == 0;
     s.keys_in = w.keys[(p + 1) & 1];
@@ -898,8 +892,8 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, 
       const cudaError_t e = cudaMemsetAsync(s.next_counts, 0, static_cast<size_t>(s.sort_blocks) * 4 << s.width, stream);
       if (e != cudaSuccess) return e;
     }
-    s.zero = share_of(rest, p + 1 < passes ? a.vocab / passes : a.vocab, sms, kSortThreads / 32);
-    sort_move_kernel<<<s.zero.blocks + s.sort_blocks, kSortThreads, 0, stream>>>(s);
+    s.zero = share_of(rest, p + 1 < passes ? a.vocab / passes : a.vocab);
+    sort_move_kernel<<<s.sort_blocks + s.zero.blocks, kSortThreads, 0, stream>>>(s);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
@@ -932,10 +926,10 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     s.chunk_sums = w.chunk_sums;
     const int64_t items = a.n_ids / kChunk * s.tiles;
     const int64_t grid = (items + 7) / 8 < sms * 5 ? (items + 7) / 8 : sms * 5;
-    chunk_sums_kernel<DT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(s);
+    s.zero = share_of(rest, (rest.end - rest.begin) / 2);
+    chunk_sums_kernel<DT, VEC><<<static_cast<unsigned>(grid) + s.zero.blocks, 256, 0, stream>>>(s);
   }
-  s.ids = ids_of(a);
-  s.zero = share_of(rest, rest.end - rest.begin, sms, 8);
+  s.zero = share_of(rest, rest.end - rest.begin);
   const int64_t max_long = a.n_ids / kLongRun * s.tiles;
   s.long_blocks = static_cast<unsigned>(!chunks ? (a.n_ids + kLongRun - 1) / kLongRun * s.tiles : max_long < 2 * sms ? max_long : 2 * sms);
   const auto finish = [&](auto kern, int vectors, size_t smem) {
@@ -948,7 +942,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * tiles < sms * per_sm * 8 * 4) s.group /= 2;
     const int64_t items = (a.n_ids + s.group - 1) / s.group * tiles;
     const int64_t token_blocks = (items + 7) / 8 < sms * per_sm ? (items + 7) / 8 : sms * per_sm;
-    kern<<<static_cast<unsigned>(s.zero.blocks + s.long_blocks + token_blocks), 256, smem, stream>>>(s);
+    kern<<<static_cast<unsigned>(s.long_blocks + token_blocks) + s.zero.blocks, 256, smem, stream>>>(s);
     return cudaGetLastError();
   };
   if constexpr (VEC > 1) {
@@ -964,7 +958,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     if (enough(2, 8)) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
     return finish(row_stream_kernel<DT, DTO, ACC, 1>, 1, kSmem);
   } else {
-    return finish(row_sums_any_kernel<DT, DTO, ACC>, 1, kMarkWords * 4);
+    return finish(row_sums_any_kernel<DT, DTO, ACC>, 1, 8 * 32 * 4);
   }
 }
 
