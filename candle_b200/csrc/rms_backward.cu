@@ -35,7 +35,7 @@ __device__ __forceinline__ float2 row_factors(float sum_xx, float sum_gax, int n
   return make_float2(r, r * (r * (r * __fdiv_rn(sum_gax, static_cast<float>(n)))));
 }
 
-// ---- any shape, any alignment: three passes -----------------------------------------------------------------
+// ---- rows too long for the kernels below: three passes, element by element ----------------------------------------
 template <int DT>
 __global__ void __launch_bounds__(kThreads) factors_kernel(const RmsBackwardArgs a, float2* factors) {
   __shared__ float scratch[2 * kThreads / 32];
@@ -105,15 +105,17 @@ __global__ void __launch_bounds__(kSumWarps * 32) sum_partials_kernel(const floa
 
 int max_partials() { return 4 * sm_count(); }
 
-// ---- whole 16-byte vectors: one pass -----------------------------------------------------------------------------
-// TPR threads take a row, VPT vectors each (columns fixed per thread, so dalpha accumulates in registers); a CTA works on
-// kThreads / TPR rows at a time and walks over the rows persistently.  Every thread brings its own vectors of the rows
-// to come into its own slots of shared memory by asynchronous copies, kStages - 1 rows ahead, and reads back only
-// what it copied itself: no barrier guards the ring, and the only one per row is that of the row sums (none for rows
-// of up to 32 threads).
-template <int VPT>
+// ---- one pass ----------------------------------------------------------------------------------------------------
+// TPR threads take a row, up to 64 bytes of it each, as vectors of VB bytes (the widest of 16, 8 and 4 that rows and
+// pointers are aligned to; columns fixed per thread, so dalpha accumulates in registers).  A CTA works on kThreads / TPR
+// rows at a time and walks over the rows persistently.  Every thread brings its own vectors of the rows to come into
+// its own slots of shared memory by asynchronous copies, kStages - 1 rows ahead, and reads back only what it copied
+// itself: no barrier guards the ring, and the only one per row is that of the row sums (none for rows of up to 32
+// threads).
+// U: 16-byte units per thread.
+template <int U>
 struct Ring {
-  static constexpr int kStages = VPT >= 3 ? 2 : 4;
+  static constexpr int kStages = U >= 3 ? 2 : 4;
 };
 
 template <int PENDING>
@@ -121,26 +123,109 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
+// A vector of VB bytes in shared memory and what it holds, as pairs.
+template <int VB>
+struct VecOf;
+template <>
+struct VecOf<16> {
+  using type = uint4;
+};
+template <>
+struct VecOf<8> {
+  using type = uint2;
+};
+template <>
+struct VecOf<4> {
+  using type = uint32_t;
+};
+template <int VB>
+__device__ __forceinline__ void copy_async(void* slot, const void* src) {
+  if constexpr (VB == 16) cp_async16(slot, src);
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(slot)), "l"(src), "n"(VB) : "memory");
+}
+template <int DT, int VB>
+__device__ __forceinline__ void widen(const typename VecOf<VB>::type& v, F2 (&f)[VB / Elem<DT>::kBytes / 2]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+  for (int j = 0; j < VB / Elem<DT>::kBytes / 2; ++j) {
+    if constexpr (DT == kDtF32) {
+      f[j] = pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    } else {
+      const float2 t = unpack2<DT>(w[j]);
+      f[j] = pair(t.x, t.y);
+    }
+  }
+}
+template <int DT, int VB>
+__device__ __forceinline__ void store_pairs(void* to, const F2 (&f)[VB / Elem<DT>::kBytes / 2]) {
+  uint32_t w[VB / 4];
+#pragma unroll
+  for (int j = 0; j < VB / Elem<DT>::kBytes / 2; ++j) {
+    const float2 t = unpair(f[j]);
+    if constexpr (DT == kDtF32) {
+      w[2 * j] = __float_as_uint(t.x);
+      w[2 * j + 1] = __float_as_uint(t.y);
+    } else {
+      w[j] = pack2<DT>(t.x, t.y);
+    }
+  }
+  if constexpr (VB == 16) stg_stream(static_cast<uint4*>(to), make_uint4(w[0], w[1], w[2], w[3]));
+  else if constexpr (VB == 8) asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(to), "r"(w[0]), "r"(w[1]) : "memory");
+  else asm volatile("st.global.cs.u32 [%0], %1;" ::"l"(to), "r"(w[0]) : "memory");
+}
+
 struct FastArgs {
   RmsBackwardArgs a;
   float* partials;  // [grid][n]
-  int tpr_shift, V;
+  int tpr_shift, V; // threads per row, vectors per row
 };
 
 constexpr int kScratchBytes = 2 * kThreads / 32 * 8;
 
-template <int DT, int VPT, bool SUM>
+// The row sums (x^2, g alpha x) over the tpr threads of a row, to all of them.  `scratch` is [2][warps]; a CTA's calls
+// use its halves in turn, since a thread may still be reading the last call's.
+__device__ __forceinline__ float2 row_sums(float2 sums, int tpr, int sub, float2* scratch, int& turn) {
+  for (int o = tpr < 32 ? tpr >> 1 : 16; o > 0; o >>= 1) {
+    sums.x += __shfl_xor_sync(0xFFFFFFFFu, sums.x, o);
+    sums.y += __shfl_xor_sync(0xFFFFFFFFu, sums.y, o);
+  }
+  if (tpr > 32) {
+    if ((threadIdx.x & 31) == 0) scratch[turn + (threadIdx.x >> 5)] = sums;
+    __syncthreads();
+    const int warps = tpr >> 5, first = sub * warps;
+    sums = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < warps; ++i) {
+      sums.x += scratch[turn + first + i].x;
+      sums.y += scratch[turn + first + i].y;
+    }
+    turn ^= kThreads / 32;
+  }
+  return sums;
+}
+
+// Adds the lines [group][n] of this CTA's row groups into its line of the partial sums.
+__device__ __forceinline__ void add_groups(const float* line, int groups, int n, float* partials) {
+  __syncthreads();
+  for (int c = threadIdx.x; c < n; c += kThreads) {
+    float t = line[c];
+    for (int i = 1; i < groups; ++i) t += line[i * n + c];
+    partials[static_cast<int64_t>(blockIdx.x) * n + c] = t;
+  }
+}
+
+template <int DT, int VB, int U, bool SUM>
 __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int P2 = Elem<DT>::kPerVec / 2, kInputs = SUM ? 3 : 2, kStages = Ring<VPT>::kStages;
-  float2* scratch = reinterpret_cast<float2*>(shared);             // [2][warps]
-  uint4* ring = reinterpret_cast<uint4*>(shared + kScratchBytes);  // [stage][input][vector][thread]
+  using V = typename VecOf<VB>::type;
+  constexpr int P2 = VB / Elem<DT>::kBytes / 2, kInputs = SUM ? 3 : 2, kStages = Ring<U>::kStages, VPT = U * 16 / VB;
+  float2* scratch = reinterpret_cast<float2*>(shared);     // [2][warps]
+  V* ring = reinterpret_cast<V*>(shared + kScratchBytes);  // [stage][input][vector][thread]
   const RmsBackwardArgs& a = f.a;
   const int tpr = 1 << f.tpr_shift, sub = threadIdx.x >> f.tpr_shift, at0 = threadIdx.x & (tpr - 1);
   const int rows_at_once = kThreads >> f.tpr_shift;
-  const int V = f.V;
+  const int n_vec = f.V;
   const float inv_n = 1.0f / static_cast<float>(a.n);
-  const uint4* src[3] = {static_cast<const uint4*>(a.x), static_cast<const uint4*>(a.grad), static_cast<const uint4*>(a.grad_sum)};
+  const V* src[3] = {static_cast<const V*>(a.x), static_cast<const V*>(a.grad), static_cast<const V*>(a.grad_sum)};
   const int64_t n_tiles = (a.rows + rows_at_once - 1) / rows_at_once;
 
   auto fetch = [&](int64_t tile, int stage) {
@@ -150,17 +235,18 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
       for (int i = 0; i < kInputs; ++i)
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
-          if (at0 + k * tpr < V)
-            cp_async16(&ring[((stage * kInputs + i) * VPT + k) * kThreads + threadIdx.x], src[i] + row * V + at0 + k * tpr);
+          if (at0 + k * tpr < n_vec)
+            copy_async<VB>(&ring[((stage * kInputs + i) * VPT + k) * kThreads + threadIdx.x], src[i] + row * n_vec + at0 + k * tpr);
     }
     cp_async_commit();
   };
 
   F2 acc[VPT][P2];
-  uint4 w[VPT];
+  V w[VPT];
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    w[k] = at0 + k * tpr < V ? __ldg(static_cast<const uint4*>(a.alpha) + at0 + k * tpr) : make_uint4(0, 0, 0, 0);
+    w[k] = V{};
+    if (at0 + k * tpr < n_vec) w[k] = __ldg(static_cast<const V*>(a.alpha) + at0 + k * tpr);
 #pragma unroll
     for (int j = 0; j < P2; ++j) acc[k][j] = 0;
   }
@@ -176,18 +262,18 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
     fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);
     ahead += gridDim.x;
     copies_wait<kStages - 1>();
-    const uint4* slot = ring + stage * kInputs * VPT * kThreads + threadIdx.x;
+    const V* slot = ring + stage * kInputs * VPT * kThreads + threadIdx.x;
     stage = stage == kStages - 1 ? 0 : stage + 1;
     const int64_t row = tile * rows_at_once + sub;
     const bool live = row < a.rows;
     F2 xx = 0, gax = 0;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      if (!live || at0 + k * tpr >= V) continue;
+      if (!live || at0 + k * tpr >= n_vec) continue;
       F2 x[P2], g[P2], u[P2];
-      vec_to_pairs<DT>(slot[k * kThreads], x);
-      vec_to_pairs<DT>(slot[(VPT + k) * kThreads], g);
-      vec_to_pairs<DT>(w[k], u);
+      widen<DT, VB>(slot[k * kThreads], x);
+      widen<DT, VB>(slot[(VPT + k) * kThreads], g);
+      widen<DT, VB>(w[k], u);
 #pragma unroll
       for (int j = 0; j < P2; ++j) {
         xx = fma2(x[j], x[j], xx);
@@ -195,33 +281,17 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
       }
     }
     const float2 t1 = unpair(xx), t2 = unpair(gax);
-    float2 sums = make_float2(t1.x + t1.y, t2.x + t2.y);
-    for (int o = tpr < 32 ? tpr >> 1 : 16; o > 0; o >>= 1) {
-      sums.x += __shfl_xor_sync(0xFFFFFFFFu, sums.x, o);
-      sums.y += __shfl_xor_sync(0xFFFFFFFFu, sums.y, o);
-    }
-    if (tpr > 32) {
-      if ((threadIdx.x & 31) == 0) scratch[turn + (threadIdx.x >> 5)] = sums;
-      __syncthreads();
-      const int warps = tpr >> 5, first = sub * warps;
-      sums = make_float2(0.0f, 0.0f);
-      for (int i = 0; i < warps; ++i) {
-        sums.x += scratch[turn + first + i].x;
-        sums.y += scratch[turn + first + i].y;
-      }
-      turn ^= kThreads / 32;  // the next row's sums go elsewhere: a thread may still be reading these
-    }
+    const float2 sums = row_sums(make_float2(t1.x + t1.y, t2.x + t2.y), tpr, sub, scratch, turn);
     const float r = rsqrtf(fmaf(sums.x, inv_n, a.eps));
     const float along = -r * (r * (r * (sums.y * inv_n)));
     const F2 r2 = pair(r, r), along2 = pair(along, along);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      if (!live || at0 + k * tpr >= V) continue;
-      F2 x[P2], g[P2], u[P2];
-      vec_to_pairs<DT>(slot[k * kThreads], x);
-      vec_to_pairs<DT>(slot[(VPT + k) * kThreads], g);
-      vec_to_pairs<DT>(w[k], u);
-      F2 d[P2];
+      if (!live || at0 + k * tpr >= n_vec) continue;
+      F2 x[P2], g[P2], u[P2], d[P2];
+      widen<DT, VB>(slot[k * kThreads], x);
+      widen<DT, VB>(slot[(VPT + k) * kThreads], g);
+      widen<DT, VB>(w[k], u);
 #pragma unroll
       for (int j = 0; j < P2; ++j) {
         const F2 gr = mul2(g[j], r2);
@@ -230,11 +300,11 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
       }
       if constexpr (SUM) {
         F2 e[P2];
-        vec_to_pairs<DT>(slot[(2 * VPT + k) * kThreads], e);
+        widen<DT, VB>(slot[(2 * VPT + k) * kThreads], e);
 #pragma unroll
         for (int j = 0; j < P2; ++j) d[j] = add2(d[j], e[j]);
       }
-      stg_stream(static_cast<uint4*>(a.dx) + row * V + at0 + k * tpr, pairs_to_vec<DT>(d));
+      store_pairs<DT, VB>(static_cast<V*>(a.dx) + row * n_vec + at0 + k * tpr, d);
     }
   }
 
@@ -243,29 +313,62 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
   float* line = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    if (at0 + k * tpr >= V) continue;
+    if (at0 + k * tpr >= n_vec) continue;
 #pragma unroll
     for (int j = 0; j < P2; ++j)
       *reinterpret_cast<F2*>(line + sub * a.n + (at0 + k * tpr) * 2 * P2 + 2 * j) = acc[k][j];
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.n; c += kThreads) {
-    float t = line[c];
-    for (int i = 1; i < rows_at_once; ++i) t += line[i * a.n + c];
-    f.partials[static_cast<int64_t>(blockIdx.x) * a.n + c] = t;
-  }
+  add_groups(line, rows_at_once, a.n, f.partials);
 }
 
-template <int DT, int VPT, bool SUM>
-cudaError_t launch_rows(const FastArgs& f, cudaStream_t stream) {
-  auto kern = rows_kernel<DT, VPT, SUM>;
-  const size_t input = static_cast<size_t>(Ring<VPT>::kStages) * VPT * kThreads * 16;
-  const size_t smem = kScratchBytes + input * (SUM ? 3 : 2);
+// Rows of any alignment, up to E elements per thread, read from memory for the sums and again (from cache) for dx.
+template <int DT, int E, bool SUM>
+__global__ void __launch_bounds__(kThreads, 2) rows_any_kernel(const FastArgs f) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  float2* scratch = reinterpret_cast<float2*>(shared);
+  float* line = reinterpret_cast<float*>(shared + kScratchBytes);
+  const RmsBackwardArgs& a = f.a;
+  const int tpr = 1 << f.tpr_shift, sub = threadIdx.x >> f.tpr_shift, at0 = threadIdx.x & (tpr - 1);
+  const int rows_at_once = kThreads >> f.tpr_shift;
+  const float inv_n = 1.0f / static_cast<float>(a.n);
+  float acc[E] = {};
+  int turn = 0;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * rows_at_once; first < a.rows; first += static_cast<int64_t>(gridDim.x) * rows_at_once) {
+    const int64_t row = first + sub, base = row * a.n;
+    const bool live = row < a.rows;
+    float xx = 0.0f, gax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int c = at0 + k * tpr;
+      if (!live || c >= a.n) continue;
+      const float x = load_elem<DT>(a.x, base + c);
+      xx = fmaf(x, x, xx);
+      gax = fmaf(load_elem<DT>(a.grad, base + c) * load_elem<DT>(a.alpha, c), x, gax);
+    }
+    const float2 sums = row_sums(make_float2(xx, gax), tpr, sub, scratch, turn);
+    const float r = rsqrtf(fmaf(sums.x, inv_n, a.eps));
+    const float along = -r * (r * (r * (sums.y * inv_n)));
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int c = at0 + k * tpr;
+      if (!live || c >= a.n) continue;
+      const float x = load_elem<DT>(a.x, base + c), gr = load_elem<DT>(a.grad, base + c) * r;
+      acc[k] = fmaf(gr, x, acc[k]);
+      float d = fmaf(gr, load_elem<DT>(a.alpha, c), x * along);
+      if constexpr (SUM) d += load_elem<DT>(a.grad_sum, base + c);
+      store_elem<DT>(a.dx, base + c, d);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < E; ++k)
+    if (at0 + k * tpr < a.n) line[sub * a.n + at0 + k * tpr] = acc[k];
+  add_groups(line, rows_at_once, a.n, f.partials);
+}
+
+// The same grid with and without grad_sum (per_sm: what fits with it), so that dalpha is summed in the same order.
+template <typename K>
+cudaError_t launch_persistent(K kern, const FastArgs& f, size_t smem, int per_sm, cudaStream_t stream) {
   cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), kThreads, smem, -1, nullptr);
-  if (e != cudaSuccess) return e;
-  // with and without grad_sum the same grid, so that dalpha is summed in the same order
-  int per_sm = 1;
-  e = kernel_launch_config(reinterpret_cast<const void*>(rows_kernel<DT, VPT, true>), kThreads, kScratchBytes + input * 3, -1, &per_sm);
   if (e != cudaSuccess) return e;
   const int rows_at_once = kThreads >> f.tpr_shift;
   int64_t grid = static_cast<int64_t>(sm_count()) * per_sm;
@@ -277,25 +380,51 @@ cudaError_t launch_rows(const FastArgs& f, cudaStream_t stream) {
   return e != cudaSuccess ? e : launch_sum_partials(f.partials, static_cast<int>(grid), f.a.n, f.a.dalpha, f.a.n, nullptr, stream);
 }
 
-// The fewest threads per row (8 .. 256) that leave at most four vectors to each; false: the row is too long.
-template <int DT>
+template <int DT, int VB, int U>
+cudaError_t launch_rows(const FastArgs& f, cudaStream_t stream) {
+  const size_t input = static_cast<size_t>(Ring<U>::kStages) * U * kThreads * 16;
+  int per_sm = 1;
+  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_kernel<DT, VB, U, true>), kThreads, kScratchBytes + input * 3, -1, &per_sm);
+  if (e != cudaSuccess) return e;
+  return f.a.grad_sum != nullptr ? launch_persistent(rows_kernel<DT, VB, U, true>, f, kScratchBytes + input * 3, per_sm, stream)
+                                 : launch_persistent(rows_kernel<DT, VB, U, false>, f, kScratchBytes + input * 2, per_sm, stream);
+}
+
+// The fewest threads per row (8 .. 256) that leave at most `most` vectors to each; how many that are, or more than `most`.
+int split_row(FastArgs& f, int most) {
+  const auto per_thread = [&] { return (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift; };
+  f.tpr_shift = 3;
+  while (f.tpr_shift < 8 && per_thread() > most) ++f.tpr_shift;
+  return per_thread();
+}
+
+// false: the row is too long for the vectors.
+template <int DT, int VB>
 bool launch_fast(const RmsBackwardArgs& a, float* partials, cudaStream_t stream, cudaError_t* e) {
-  FastArgs f{a, partials, 3, a.n / Elem<DT>::kPerVec};
-  while (f.tpr_shift < 8 && (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift > 4) ++f.tpr_shift;
-  const int vpt = (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift;
-  if (vpt > 4) return false;
-  const bool sum = a.grad_sum != nullptr;
-  switch (vpt) {
-    case 1: *e = sum ? launch_rows<DT, 1, true>(f, stream) : launch_rows<DT, 1, false>(f, stream); break;
-    case 2: *e = sum ? launch_rows<DT, 2, true>(f, stream) : launch_rows<DT, 2, false>(f, stream); break;
-    case 3: *e = sum ? launch_rows<DT, 3, true>(f, stream) : launch_rows<DT, 3, false>(f, stream); break;
-    default: *e = sum ? launch_rows<DT, 4, true>(f, stream) : launch_rows<DT, 4, false>(f, stream); break;
+  FastArgs f{a, partials, 3, a.n * Elem<DT>::kBytes / VB};
+  const int units = (split_row(f, 64 / VB) * VB + 15) / 16;
+  if (units > 4) return false;
+  switch (units) {
+    case 1: *e = launch_rows<DT, VB, 1>(f, stream); break;
+    case 2: *e = launch_rows<DT, VB, 2>(f, stream); break;
+    case 3: *e = launch_rows<DT, VB, 3>(f, stream); break;
+    default: *e = launch_rows<DT, VB, 4>(f, stream); break;
   }
   return true;
 }
 
+template <int DT, int E>
+cudaError_t launch_elements(const FastArgs& f, cudaStream_t stream) {
+  const size_t smem = kScratchBytes + static_cast<size_t>(kThreads) * E * 4;
+  int per_sm = 1;
+  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_any_kernel<DT, E, true>), kThreads, smem, -1, &per_sm);
+  if (e != cudaSuccess) return e;
+  return f.a.grad_sum != nullptr ? launch_persistent(rows_any_kernel<DT, E, true>, f, smem, per_sm, stream)
+                                 : launch_persistent(rows_any_kernel<DT, E, false>, f, smem, per_sm, stream);
+}
+
 template <int DT>
-cudaError_t launch_any(const RmsBackwardArgs& a, float* partials, float2* factors, cudaStream_t stream) {
+cudaError_t launch_long(const RmsBackwardArgs& a, float* partials, float2* factors, cudaStream_t stream) {
   int64_t grid = static_cast<int64_t>(sm_count()) * 8;
   if (grid > a.rows) grid = a.rows;
   factors_kernel<DT><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a, factors);
@@ -305,6 +434,22 @@ cudaError_t launch_any(const RmsBackwardArgs& a, float* partials, float2* factor
   dx_kernel<DT><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a, factors);
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_sum_partials(partials, slices, a.n, a.dalpha, a.n, nullptr, stream);
+}
+
+template <int DT>
+cudaError_t launch_dt(const RmsBackwardArgs& a, float* partials, float2* factors, cudaStream_t stream) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.alpha) |
+                       reinterpret_cast<uintptr_t>(a.grad_sum) | reinterpret_cast<uintptr_t>(a.dx) |
+                       static_cast<uintptr_t>(a.n) * Elem<DT>::kBytes;
+  cudaError_t e = cudaSuccess;
+  if (at % 16 == 0 && launch_fast<DT, 16>(a, partials, stream, &e)) return e;
+  if (at % 8 == 0 && launch_fast<DT, 8>(a, partials, stream, &e)) return e;
+  if constexpr (DT != kDtF32)
+    if (at % 4 == 0 && launch_fast<DT, 4>(a, partials, stream, &e)) return e;
+  FastArgs f{a, partials, 3, a.n};
+  const int elements = split_row(f, 32);
+  if (elements > 32) return launch_long<DT>(a, partials, factors, stream);
+  return elements <= 8 ? launch_elements<DT, 8>(f, stream) : elements <= 16 ? launch_elements<DT, 16>(f, stream) : launch_elements<DT, 32>(f, stream);
 }
 
 }  // namespace
@@ -325,14 +470,10 @@ cudaError_t launch_rms_backward(int dtype, const RmsBackwardArgs& a, void* works
   float* partials = static_cast<float*>(workspace);
   float2* factors = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
                                               ((static_cast<int64_t>(max_partials()) * a.n * 4 + 15) & ~int64_t(15)));
-  const uintptr_t at = reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.alpha) |
-                       reinterpret_cast<uintptr_t>(a.grad_sum) | reinterpret_cast<uintptr_t>(a.dx);
-  const bool vectors = at % 16 == 0 && a.n % (dtype == kDtF32 ? 4 : 8) == 0;
-  cudaError_t e = cudaSuccess;
   switch (dtype) {
-    case kDtF32: return vectors && launch_fast<kDtF32>(a, partials, stream, &e) ? e : launch_any<kDtF32>(a, partials, factors, stream);
-    case kDtF16: return vectors && launch_fast<kDtF16>(a, partials, stream, &e) ? e : launch_any<kDtF16>(a, partials, factors, stream);
-    default: return vectors && launch_fast<kDtBF16>(a, partials, stream, &e) ? e : launch_any<kDtBF16>(a, partials, factors, stream);
+    case kDtF32: return launch_dt<kDtF32>(a, partials, factors, stream);
+    case kDtF16: return launch_dt<kDtF16>(a, partials, factors, stream);
+    default: return launch_dt<kDtBF16>(a, partials, factors, stream);
   }
 }
 
