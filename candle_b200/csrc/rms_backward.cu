@@ -180,7 +180,8 @@ struct FastArgs {
   int tpr_shift, V; // threads per row, vectors per row
 };
 
-constexpr int kScratchBytes = 2 * kThreads / 32 * 8;
+constexpr int kWideThreads = 512;  // CTAs for rows that 256 threads do not hold
+constexpr int kScratchBytes = 2 * kWideThreads / 32 * 8;
 
 // The row sums (x^2, g alpha x) over the tpr threads of a row, to all of them.  `scratch` is [2][warps]; a CTA's calls
 // use its halves in turn, since a thread may still be reading the last call's.
@@ -198,7 +199,7 @@ __device__ __forceinline__ float2 row_sums(float2 sums, int tpr, int sub, float2
       sums.x += scratch[turn + first + i].x;
       sums.y += scratch[turn + first + i].y;
     }
-    turn ^= kThreads / 32;
+    turn ^= blockDim.x / 32;
   }
   return sums;
 }
@@ -206,15 +207,15 @@ __device__ __forceinline__ float2 row_sums(float2 sums, int tpr, int sub, float2
 // Adds the lines [group][n] of this CTA's row groups into its line of the partial sums.
 __device__ __forceinline__ void add_groups(const float* line, int groups, int n, float* partials) {
   __syncthreads();
-  for (int c = threadIdx.x; c < n; c += kThreads) {
+  for (int c = threadIdx.x; c < n; c += blockDim.x) {
     float t = line[c];
     for (int i = 1; i < groups; ++i) t += line[i * n + c];
     partials[static_cast<int64_t>(blockIdx.x) * n + c] = t;
   }
 }
 
-template <int DT, int VB, int U, bool SUM>
-__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
+template <int DT, int VB, int U, bool SUM, int T>
+__global__ void __launch_bounds__(T, 512 / T) rows_kernel(const FastArgs f) {
   extern __shared__ __align__(16) unsigned char shared[];
   using V = typename VecOf<VB>::type;
   constexpr int P2 = VB / Elem<DT>::kBytes / 2, kInputs = SUM ? 3 : 2, kStages = Ring<U>::kStages, VPT = U * 16 / VB;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
   V* ring = reinterpret_cast<V*>(shared + kScratchBytes);  // [stage][input][vector][thread]
   const RmsBackwardArgs& a = f.a;
   const int tpr = 1 << f.tpr_shift, sub = threadIdx.x >> f.tpr_shift, at0 = threadIdx.x & (tpr - 1);
-  const int rows_at_once = kThreads >> f.tpr_shift;
+  const int rows_at_once = T >> f.tpr_shift;
   const int n_vec = f.V;
   const float inv_n = 1.0f / static_cast<float>(a.n);
   const V* src[3] = {static_cast<const V*>(a.x), static_cast<const V*>(a.grad), static_cast<const V*>(a.grad_sum)};
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
           if (at0 + k * tpr < n_vec)
-            copy_async<VB>(&ring[((stage * kInputs + i) * VPT + k) * kThreads + threadIdx.x], src[i] + row * n_vec + at0 + k * tpr);
+            copy_async<VB>(&ring[((stage * kInputs + i) * VPT + k) * T + threadIdx.x], src[i] + row * n_vec + at0 + k * tpr);
     }
     cp_async_commit();
   };
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
     fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);
     ahead += gridDim.x;
     copies_wait<kStages - 1>();
-    const V* slot = ring + stage * kInputs * VPT * kThreads + threadIdx.x;
+    const V* slot = ring + stage * kInputs * VPT * T + threadIdx.x;
     stage = stage == kStages - 1 ? 0 : stage + 1;
     const int64_t row = tile * rows_at_once + sub;
     const bool live = row < a.rows;
@@ -271,8 +272,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
     for (int k = 0; k < VPT; ++k) {
       if (!live || at0 + k * tpr >= n_vec) continue;
       F2 x[P2], g[P2], u[P2];
-      widen<DT, VB>(slot[k * kThreads], x);
-      widen<DT, VB>(slot[(VPT + k) * kThreads], g);
+      widen<DT, VB>(slot[k * T], x);
+      widen<DT, VB>(slot[(VPT + k) * T], g);
       widen<DT, VB>(w[k], u);
 #pragma unroll
       for (int j = 0; j < P2; ++j) {
@@ -289,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
     for (int k = 0; k < VPT; ++k) {
       if (!live || at0 + k * tpr >= n_vec) continue;
       F2 x[P2], g[P2], u[P2], d[P2];
-      widen<DT, VB>(slot[k * kThreads], x);
-      widen<DT, VB>(slot[(VPT + k) * kThreads], g);
+      widen<DT, VB>(slot[k * T], x);
+      widen<DT, VB>(slot[(VPT + k) * T], g);
       widen<DT, VB>(w[k], u);
 #pragma unroll
       for (int j = 0; j < P2; ++j) {
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
       }
       if constexpr (SUM) {
         F2 e[P2];
-        widen<DT, VB>(slot[(2 * VPT + k) * kThreads], e);
+        widen<DT, VB>(slot[(2 * VPT + k) * T], e);
 #pragma unroll
         for (int j = 0; j < P2; ++j) d[j] = add2(d[j], e[j]);
       }
@@ -321,29 +322,73 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const FastArgs f) {
   add_groups(line, rows_at_once, a.n, f.partials);
 }
 
-// Rows of any alignment, up to E elements per thread, read from memory for the sums and again (from cache) for dx.
+// Rows of any alignment, up to E elements per thread.  The rows of a visit lie next to one another in memory and come
+// into shared memory as they lie, whole 16-byte vectors by asynchronous copies, the ends by elements, while the visit
+// before is worked on; the threads then pick their elements.  (Loads of single elements out of memory leave too few
+// bytes in flight: 60000 rows of 4097 bf16 took 2.6 ms.)
+// Bytes of a visit's rows in shared memory: they begin where their first byte does within 16.
+__host__ __device__ inline int64_t visit_bytes(int64_t rows, int n, int elem) { return (rows * n * elem + 15 + 15) / 16 * 16; }
+
+template <int DT>
+__device__ __forceinline__ void bring_rows(unsigned char* to, const void* from, int64_t bytes) {
+  using T = typename Elem<DT>::type;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(from), end = begin + bytes;
+  const uintptr_t base = begin & ~uintptr_t(15), whole = (begin + 15) & ~uintptr_t(15), behind = end & ~uintptr_t(15);
+  for (uintptr_t p = whole + threadIdx.x * 16; p + 16 <= end; p += kThreads * 16) cp_async16(to + (p - base), reinterpret_cast<const void*>(p));
+  // fewer than 16 bytes at either end; all of them where no whole vector lies between
+  const uintptr_t head_end = whole < end ? whole : end, tail = behind > head_end ? behind : head_end;
+  for (uintptr_t p = begin + threadIdx.x * sizeof(T); p < head_end; p += kThreads * sizeof(T)) *reinterpret_cast<T*>(to + (p - base)) = *reinterpret_cast<const T*>(p);
+  for (uintptr_t p = tail + threadIdx.x * sizeof(T); p < end; p += kThreads * sizeof(T)) *reinterpret_cast<T*>(to + (p - base)) = *reinterpret_cast<const T*>(p);
+}
+
 template <int DT, int E, bool SUM>
 __global__ void __launch_bounds__(kThreads, 2) rows_any_kernel(const FastArgs f) {
   extern __shared__ __align__(16) unsigned char shared[];
-  float2* scratch = reinterpret_cast<float2*>(shared);
-  float* line = reinterpret_cast<float*>(shared + kScratchBytes);
+  constexpr int kInputs = SUM ? 3 : 2, kBytes = Elem<DT>::kBytes;
   const RmsBackwardArgs& a = f.a;
   const int tpr = 1 << f.tpr_shift, sub = threadIdx.x >> f.tpr_shift, at0 = threadIdx.x & (tpr - 1);
   const int rows_at_once = kThreads >> f.tpr_shift;
   const float inv_n = 1.0f / static_cast<float>(a.n);
-  float acc[E] = {};
-  int turn = 0;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * rows_at_once; first < a.rows; first += static_cast<int64_t>(gridDim.x) * rows_at_once) {
-    const int64_t row = first + sub, base = row * a.n;
-    const bool live = row < a.rows;
+  float2* scratch = reinterpret_cast<float2*>(shared);
+  unsigned char* ring = shared + kScratchBytes;  // [stage][input][visit_bytes]
+  const int64_t piece = visit_bytes(rows_at_once, a.n, kBytes);
+  const void* src[3] = {a.x, a.grad, a.grad_sum};
+  auto address = [&](int i, int64_t row) { return static_cast<const unsigned char*>(src[i]) + row * a.n * kBytes; };
+  auto bring = [&](int64_t first, int stage) {
+    if (first < a.rows) {
+      const int64_t rows = a.rows - first < rows_at_once ? a.rows - first : rows_at_once;
+#pragma unroll
+      for (int i = 0; i < kInputs; ++i) bring_rows<DT>(ring + (stage * kInputs + i) * piece, address(i, first), rows * a.n * kBytes);
+    }
+    cp_async_commit();
+  };
+
+  float acc[E] = {}, w[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) w[k] = at0 + k * tpr < a.n ? load_elem<DT>(a.alpha, at0 + k * tpr) : 0.0f;
+  int turn = 0, stage = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rows_at_once;
+  int64_t first = static_cast<int64_t>(blockIdx.x) * rows_at_once;
+  bring(first, 0);
+  for (; first < a.rows; first += step) {
+    cp_async_wait_all();
+    __syncthreads();  // the visit's rows are here, and the visit before is done with the other stage
+    bring(first + step, stage ^ 1);
+    const int64_t row = first + sub;
+    const int n = row < a.rows ? a.n : 0;
+    const unsigned char* at[3];
+#pragma unroll
+    for (int i = 0; i < kInputs; ++i)
+      at[i] = ring + (stage * kInputs + i) * piece + (reinterpret_cast<uintptr_t>(address(i, first)) & 15) + static_cast<int64_t>(sub) * a.n * kBytes;
+    stage ^= 1;
     float xx = 0.0f, gax = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
       const int c = at0 + k * tpr;
-      if (!live || c >= a.n) continue;
-      const float x = load_elem<DT>(a.x, base + c);
+      if (c >= n) continue;
+      const float x = load_elem<DT>(at[0], c);
       xx = fmaf(x, x, xx);
-      gax = fmaf(load_elem<DT>(a.grad, base + c) * load_elem<DT>(a.alpha, c), x, gax);
+      gax = fmaf(load_elem<DT>(at[1], c) * w[k], x, gax);
     }
     const float2 sums = row_sums(make_float2(xx, gax), tpr, sub, scratch, turn);
     const float r = rsqrtf(fmaf(sums.x, inv_n, a.eps));
@@ -351,14 +396,16 @@ __global__ void __launch_bounds__(kThreads, 2) rows_any_kernel(const FastArgs f)
 #pragma unroll
     for (int k = 0; k < E; ++k) {
       const int c = at0 + k * tpr;
-      if (!live || c >= a.n) continue;
-      const float x = load_elem<DT>(a.x, base + c), gr = load_elem<DT>(a.grad, base + c) * r;
+      if (c >= n) continue;
+      const float x = load_elem<DT>(at[0], c), gr = load_elem<DT>(at[1], c) * r;
       acc[k] = fmaf(gr, x, acc[k]);
-      float d = fmaf(gr, load_elem<DT>(a.alpha, c), x * along);
-      if constexpr (SUM) d += load_elem<DT>(a.grad_sum, base + c);
-      store_elem<DT>(a.dx, base + c, d);
+      float d = fmaf(gr, w[k], x * along);
+      if constexpr (SUM) d += load_elem<DT>(at[2], c);
+      store_elem<DT>(a.dx, row * a.n + c, d);
     }
   }
+  __syncthreads();
+  float* line = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int k = 0; k < E; ++k)
     if (at0 + k * tpr < a.n) line[sub * a.n + at0 + k * tpr] = acc[k];
@@ -367,34 +414,35 @@ __global__ void __launch_bounds__(kThreads, 2) rows_any_kernel(const FastArgs f)
 
 // The same grid with and without grad_sum (per_sm: what fits with it), so that dalpha is summed in the same order.
 template <typename K>
-cudaError_t launch_persistent(K kern, const FastArgs& f, size_t smem, int per_sm, cudaStream_t stream) {
-  cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), kThreads, smem, -1, nullptr);
+cudaError_t launch_persistent(K kern, const FastArgs& f, int threads, size_t smem, int per_sm, cudaStream_t stream) {
+  cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), threads, smem, -1, nullptr);
   if (e != cudaSuccess) return e;
-  const int rows_at_once = kThreads >> f.tpr_shift;
+  const int rows_at_once = threads >> f.tpr_shift;
   int64_t grid = static_cast<int64_t>(sm_count()) * per_sm;
   if (grid > max_partials()) grid = max_partials();
   const int64_t tiles = (f.a.rows + rows_at_once - 1) / rows_at_once;
   if (grid > tiles) grid = tiles;
-  kern<<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(f);
+  kern<<<static_cast<unsigned>(grid), threads, smem, stream>>>(f);
   e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_sum_partials(f.partials, static_cast<int>(grid), f.a.n, f.a.dalpha, f.a.n, nullptr, stream);
 }
 
-template <int DT, int VB, int U>
+template <int DT, int VB, int U, int T>
 cudaError_t launch_rows(const FastArgs& f, cudaStream_t stream) {
-  const size_t input = static_cast<size_t>(Ring<U>::kStages) * U * kThreads * 16;
+  const size_t input = static_cast<size_t>(Ring<U>::kStages) * U * T * 16;
   int per_sm = 1;
-  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_kernel<DT, VB, U, true>), kThreads, kScratchBytes + input * 3, -1, &per_sm);
+  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_kernel<DT, VB, U, true, T>), T, kScratchBytes + input * 3, -1, &per_sm);
   if (e != cudaSuccess) return e;
-  return f.a.grad_sum != nullptr ? launch_persistent(rows_kernel<DT, VB, U, true>, f, kScratchBytes + input * 3, per_sm, stream)
-                                 : launch_persistent(rows_kernel<DT, VB, U, false>, f, kScratchBytes + input * 2, per_sm, stream);
+  return f.a.grad_sum != nullptr ? launch_persistent(rows_kernel<DT, VB, U, true, T>, f, T, kScratchBytes + input * 3, per_sm, stream)
+                                 : launch_persistent(rows_kernel<DT, VB, U, false, T>, f, T, kScratchBytes + input * 2, per_sm, stream);
 }
 
-// The fewest threads per row (8 .. 256) that leave at most `most` vectors to each; how many that are, or more than `most`.
-int split_row(FastArgs& f, int most) {
+// The fewest threads per row (8 .. max_threads) that leave at most `most` vectors to each; how many that are, or more
+// than `most`.
+int split_row(FastArgs& f, int most, int max_threads) {
   const auto per_thread = [&] { return (f.V + (1 << f.tpr_shift) - 1) >> f.tpr_shift; };
   f.tpr_shift = 3;
-  while (f.tpr_shift < 8 && per_thread() > most) ++f.tpr_shift;
+  while ((1 << f.tpr_shift) < max_threads && per_thread() > most) ++f.tpr_shift;
   return per_thread();
 }
 
@@ -402,25 +450,29 @@ int split_row(FastArgs& f, int most) {
 template <int DT, int VB>
 bool launch_fast(const RmsBackwardArgs& a, float* partials, cudaStream_t stream, cudaError_t* e) {
   FastArgs f{a, partials, 3, a.n * Elem<DT>::kBytes / VB};
-  const int units = (split_row(f, 64 / VB) * VB + 15) / 16;
+  const int units = (split_row(f, 64 / VB, kWideThreads) * VB + 15) / 16;
   if (units > 4) return false;
+  if (f.tpr_shift == 9) {  // more than half of what the 512 threads hold
+    *e = units == 3 ? launch_rows<DT, VB, 3, kWideThreads>(f, stream) : launch_rows<DT, VB, 4, kWideThreads>(f, stream);
+    return true;
+  }
   switch (units) {
-    case 1: *e = launch_rows<DT, VB, 1>(f, stream); break;
-    case 2: *e = launch_rows<DT, VB, 2>(f, stream); break;
-    case 3: *e = launch_rows<DT, VB, 3>(f, stream); break;
-    default: *e = launch_rows<DT, VB, 4>(f, stream); break;
+    case 1: *e = launch_rows<DT, VB, 1, kThreads>(f, stream); break;
+    case 2: *e = launch_rows<DT, VB, 2, kThreads>(f, stream); break;
+    case 3: *e = launch_rows<DT, VB, 3, kThreads>(f, stream); break;
+    default: *e = launch_rows<DT, VB, 4, kThreads>(f, stream); break;
   }
   return true;
 }
 
 template <int DT, int E>
 cudaError_t launch_elements(const FastArgs& f, cudaStream_t stream) {
-  const size_t smem = kScratchBytes + static_cast<size_t>(kThreads) * E * 4;
+  const size_t input = 2 * static_cast<size_t>(visit_bytes(kThreads >> f.tpr_shift, f.a.n, Elem<DT>::kBytes));
   int per_sm = 1;
-  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_any_kernel<DT, E, true>), kThreads, smem, -1, &per_sm);
+  const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(rows_any_kernel<DT, E, true>), kThreads, kScratchBytes + 3 * input, -1, &per_sm);
   if (e != cudaSuccess) return e;
-  return f.a.grad_sum != nullptr ? launch_persistent(rows_any_kernel<DT, E, true>, f, smem, per_sm, stream)
-                                 : launch_persistent(rows_any_kernel<DT, E, false>, f, smem, per_sm, stream);
+  return f.a.grad_sum != nullptr ? launch_persistent(rows_any_kernel<DT, E, true>, f, kThreads, kScratchBytes + 3 * input, per_sm, stream)
+                                 : launch_persistent(rows_any_kernel<DT, E, false>, f, kThreads, kScratchBytes + 2 * input, per_sm, stream);
 }
 
 template <int DT>
@@ -447,9 +499,11 @@ cudaError_t launch_dt(const RmsBackwardArgs& a, float* partials, float2* factors
   if constexpr (DT != kDtF32)
     if (at % 4 == 0 && launch_fast<DT, 4>(a, partials, stream, &e)) return e;
   FastArgs f{a, partials, 3, a.n};
-  const int elements = split_row(f, 32);
+  const int elements = split_row(f, 32, kThreads);
   if (elements > 32) return launch_long<DT>(a, partials, factors, stream);
-  return elements <= 8 ? launch_elements<DT, 8>(f, stream) : elements <= 16 ? launch_elements<DT, 16>(f, stream) : launch_elements<DT, 32>(f, stream);
+  if (elements <= 8) return launch_elements<DT, 8>(f, stream);
+  if (elements <= 16) return launch_elements<DT, 16>(f, stream);
+  return elements <= 24 ? launch_elements<DT, 24>(f, stream) : launch_elements<DT, 32>(f, stream);
 }
 
 }  // namespace
