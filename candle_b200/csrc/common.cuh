@@ -387,6 +387,16 @@ __device__ __forceinline__ void cp_async_wait_pending(int pending) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Kernels that follow one another in one call (launch_dependent in launch.h): the later one's CTAs take their places while
+// the earlier one ends.  follow_previous() waits until the earlier grid is complete and its writes are visible, then lets
+// the next kernel of the call begin to do the same; every thread calls it before it touches memory.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void follow_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------------------------
 // Warp reductions.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ float warp_sum(float v) {

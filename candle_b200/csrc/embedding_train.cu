@@ -5,9 +5,9 @@
 // fixed order: no floating-point atomics, equal inputs give equal bits.  Then
 //   - chunk_sums_kernel adds up every aligned chunk of 32 sorted tokens that belongs to one id: text is skewed
 //     (the hottest id of 65536 tokens has thousands) and this is what spreads a long run over the GPU;
-//   - row_sums_kernel writes the table rows.  Work is cut by tokens, not by rows, since a few rows of a text's table
-//     have most of its tokens: a warp adds the runs that begin at a few neighbouring sorted positions, a CTA a
-//     long run (the chunk sums and the ends that do not fill a chunk).
+//   - long_runs_kernel adds these and the ends that do not fill a chunk, for runs of 64 tokens and more;
+//   - row_stream_kernel adds the other runs.  Work is cut by tokens, not by rows, since a few rows of a text's table have
+//     most of its tokens: a warp takes the runs that begin at a few neighbouring sorted positions.
 // The rows without tokens are filled with zeros by further blocks of the launches that leave the memory idle: the radix
 // sort's, or with few tokens the chunk sums' or the row sums'.
 #include "launch.h"
@@ -148,7 +148,7 @@ __device__ __forceinline__ uint32_t key_of_id(const Ids& a, int64_t i, bool repo
 // Rows without tokens.  A block fills a few neighbouring rows and ends: blocks that follow one another through memory
 // write at 7.4 TB/s, resident ones that stride over the table at 6.0 (1 GB, rows of 8 KB).
 // ---------------------------------------------------------------------------------------------
-constexpr int kFillBytes = 32 * 1024;  // per block, but at least a row
+constexpr int kFillBytes = 64 * 1024;  // per block, but at least a row (16 KB: 60 us more for 0.9 GB, the launches of the blocks)
 
 struct ZeroFill {
   unsigned char* out;      // the table's gradient
@@ -271,6 +271,7 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[kSortItems], 
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs a) {
+  follow_previous();
   __shared__ uint32_t hist[kSortMaxBins];
   __shared__ uint32_t marked[kSortThreads];  // some id of each residue that was marked already, or none
   const int bins = 1 << a.width;
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs a) {
+  follow_previous();
   __shared__ uint32_t base[kSortMaxBins];
   __shared__ uint32_t totals[kSortThreads / 32];
   __shared__ uint16_t count[kSortThreads / 32][kSortMaxBins];
@@ -364,6 +366,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortArgs 
 
 // A block places 32 tokens.
 __global__ void __launch_bounds__(kRankThreads) sort_small_kernel(const SortArgs a) {
+  follow_previous();
   extern __shared__ __align__(16) uint32_t words[];
   __shared__ uint32_t part[kRankWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = static_cast<int>(a.n);
@@ -425,7 +428,6 @@ struct SumArgs {
   int units;               // VEC-element units per row
   int tiles;               // tiles of 32 units per row
   int group;               // sorted positions per warp and visit
-  unsigned long_blocks;    // the first blocks, for the long runs
   ZeroFill zero;
 };
 constexpr int kChunkBatch = 8;
@@ -453,8 +455,9 @@ __device__ __forceinline__ void write_unit(const SumArgs& a, int64_t row, int u,
 }
 
 // Lists the long runs and adds up the chunks that one id fills.
-template <int DT, int VEC>
+template <int DT, int VEC, int C>
 __global__ void __launch_bounds__(256) chunk_sums_kernel(const __grid_constant__ SumArgs a) {
+  follow_previous();
   const unsigned blocks = gridDim.x - a.zero.blocks;
   if (blockIdx.x >= blocks) return fill_rows(a.zero, blockIdx.x - blocks);
   const int lane = threadIdx.x & 31;
@@ -467,26 +470,33 @@ __global__ void __launch_bounds__(256) chunk_sums_kernel(const __grid_constant__
     const int64_t behind = i + kLongRun;  // of the 64 positions from i on
     if (behind == a.n || a.keys[behind] != key) a.long_runs[atomicAdd(a.n_long, 1u)] = make_uint2(static_cast<uint32_t>(behind), key);
   }
-  const int64_t n_items = a.n / kChunk * a.tiles;
+  const int tiles = (a.units + 32 * C - 1) / (32 * C);
+  const int64_t n_items = a.n / kChunk * tiles;
   for (int64_t item = me >> 5; item < n_items; item += threads >> 5) {
-    const int64_t c = item / a.tiles;
-    const uint32_t key = a.keys[c * kChunk + lane % kChunk], token = a.tokens[c * kChunk + lane % kChunk];
+    const int64_t c = item / tiles;
+    const uint32_t key = a.keys[c * kChunk + lane], token = a.tokens[c * kChunk + lane];
     if (key >= a.vocab || !__all_sync(0xFFFFFFFFu, key == __shfl_sync(0xFFFFFFFFu, key, 0))) continue;
-    const int u = static_cast<int>(item - c * a.tiles) * 32 + lane;
-    float acc[VEC] = {};
+    const int u0 = static_cast<int>(item - c * tiles) * (32 * C) + lane;
+    float acc[C][VEC] = {};
 #pragma unroll
     for (int t0 = 0; t0 < kChunk; t0 += kChunkBatch) {
-      Unit<DT, VEC> q[kChunkBatch];
+      Unit<DT, VEC> q[kChunkBatch][C];
 #pragma unroll
       for (int t = 0; t < kChunkBatch; ++t) {
         const int64_t at = static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, token, t0 + t)) * a.grad_stride;
-        if (u < a.units) q[t] = load_unit<DT, VEC>(a.grad, at + static_cast<int64_t>(u) * VEC);
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (u0 + 32 * j < a.units) q[t][j] = load_unit<DT, VEC>(a.grad, at + static_cast<int64_t>(u0 + 32 * j) * VEC);
       }
 #pragma unroll
       for (int t = 0; t < kChunkBatch; ++t)
-        if (u < a.units) add_unit<DT, VEC>(q[t], acc);
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (u0 + 32 * j < a.units) add_unit<DT, VEC>(q[t][j], acc[j]);
     }
-    if (u < a.units) store_floats<kDtF32, VEC>(a.chunk_sums, c * a.hidden + static_cast<int64_t>(u) * VEC, acc);
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+      if (u0 + 32 * j < a.units) store_floats<kDtF32, VEC>(a.chunk_sums, c * a.hidden + static_cast<int64_t>(u0 + 32 * j) * VEC, acc[j]);
   }
 }
 
@@ -506,58 +516,149 @@ __device__ __forceinline__ int64_t run_end(const SumArgs& a, int64_t at) {
   return hi;
 }
 
-// A long run [begin, end) of id `key`, by a CTA per tile of 32 units: the tokens before and behind its whole chunks (all
-// of them where there are no chunk sums) and the chunk sums, each warp every eighth, then the warps' parts in order.
+// acc += every step-th piece of a long run [begin, end) from `piece` on, for the unit u of its row: the tokens before and
+// behind the whole chunks (all tokens where there are no chunk sums), then the chunk sums.  The pieces come into `ring`, the
+// lane's slots of shared memory, kPieces - 1 ahead.
+constexpr int kPieces = 8;
+template <int VEC>
+struct PieceRing {
+  static constexpr int kWords = VEC > 1 ? VEC / 4 : 0;  // 16-byte words per lane and slot: VEC floats of a chunk sum
+};
+
+template <int DT, int VEC>
+__device__ __forceinline__ void add_pieces(const SumArgs& a, int64_t begin, int64_t end, int u, int64_t piece, int step,
+                                           uint4* ring, float (&acc)[VEC]) {
+  const int lane = threadIdx.x & 31;
+  int64_t first = a.chunk_sums == nullptr ? 0 : (begin + kChunk - 1) / kChunk, last = a.chunk_sums == nullptr ? 0 : end / kChunk;
+  if (first >= last) first = last = 0;
+  const int64_t head = first < last ? first * kChunk - begin : end - begin, loose = first < last ? head + end - last * kChunk : head;
+  const int64_t pieces = loose + last - first, count = piece < pieces ? (pieces - piece + step - 1) / step : 0;
+  const bool here = u < a.units;
+  uint32_t ahead = 0;  // lane l: position of the token that is piece number i - i % 32 + l of this warp
+  auto positions = [&](int64_t i) {
+    const int64_t e = piece + (i + lane) * step;
+    ahead = e < loose ? a.tokens[e < head ? begin + e : last * kChunk + (e - head)] : 0u;
+  };
+  if constexpr (VEC == 1) {
+    for (int64_t i = 0; i < count; ++i) {
+      if (i % 32 == 0) positions(i);
+      const int64_t e = piece + i * step;
+      const int64_t token = __shfl_sync(0xFFFFFFFFu, ahead, static_cast<int>(i % 32));
+      if (here) acc[0] += e < loose ? load_elem<DT>(a.grad, token * a.grad_stride + u) : a.chunk_sums[(first + e - loose) * a.hidden + u];
+    }
+  } else {
+    constexpr int kWords = PieceRing<VEC>::kWords;
+    for (int64_t i = 0; i < count + kPieces - 1; ++i) {
+      if (i < count) {
+        if (i % 32 == 0) positions(i);
+        const int64_t e = piece + i * step;
+        const int64_t token = __shfl_sync(0xFFFFFFFFu, ahead, static_cast<int>(i % 32));
+        uint4* slot = ring + static_cast<int>(i % kPieces) * (kWords * 32);
+        if (here && e < loose) {
+          cp_async16(slot, static_cast<const unsigned char*>(a.grad) + (token * a.grad_stride + static_cast<int64_t>(u) * VEC) * Elem<DT>::kBytes);
+        } else if (here) {
+          const float* sums = a.chunk_sums + (first + e - loose) * a.hidden + static_cast<int64_t>(u) * VEC;
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) cp_async16(slot + w * 32, sums + 4 * w);
+        }
+      }
+      cp_async_commit();
+      const int64_t done = i - (kPieces - 1);
+      if (done < 0) continue;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kPieces - 1) : "memory");
+      const uint4* slot = ring + static_cast<int>(done % kPieces) * (kWords * 32);
+      if (here && piece + done * step < loose) {
+        Unit<DT, VEC> q;
+        q.v = slot[0];
+        add_unit<DT, VEC>(q, acc);
+      } else if (here) {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          const uint4 v = slot[w * 32];
+          acc[4 * w] += __uint_as_float(v.x);
+          acc[4 * w + 1] += __uint_as_float(v.y);
+          acc[4 * w + 2] += __uint_as_float(v.z);
+          acc[4 * w + 3] += __uint_as_float(v.w);
+        }
+      }
+    }
+    cp_async_wait_all();
+  }
+}
+
+template <int DTO, int VEC, bool ACC>
+__device__ __forceinline__ void finish_run(const SumArgs& a, uint32_t key, int u, const float (&acc)[VEC]) {
+  if (u >= a.units) return;
+  float old[VEC] = {};
+  if constexpr (ACC) load_floats_plain<DTO, VEC>(a.out, static_cast<int64_t>(key) * a.hidden + static_cast<int64_t>(u) * VEC, old);
+  write_unit<DTO, VEC, ACC>(a, key, u, acc, old);
+}
+
+// The long runs.  With chunk sums and many of them: eight (run, tile) items per CTA at a time, a warp for each run of fewer
+// than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.
+constexpr int kWarpRun = 512;
 template <int DT, int DTO, int VEC, bool ACC>
-__device__ __noinline__ void add_long_run(const SumArgs& a, int64_t begin, int64_t end, uint32_t key, int tile, float (*part)[32 * VEC]) {
+__global__ void __launch_bounds__(256, 3) long_runs_kernel(const __grid_constant__ SumArgs a) {
+  follow_previous();
+  extern __shared__ __align__(16) unsigned char shared[];
+  float(*part)[32 * VEC] = reinterpret_cast<float(*)[32 * VEC]>(shared);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int u = tile * 32 + lane;
-  const int64_t first = a.chunk_sums == nullptr ? 0 : (begin + kChunk - 1) / kChunk, last = a.chunk_sums == nullptr ? 0 : end / kChunk;
-  // tokens outside the chunks [first, last): index e < head is begin + e, the others go on at the last chunk's end
-  const int64_t head = first == last ? end - begin : first * kChunk - begin, loose = first == last ? head : head + end - last * kChunk;
-  float acc[VEC] = {};
-  for (int64_t e = warp; e < loose; e += 8 * kTokenBatch) {
-    uint32_t token[kTokenBatch];
-    Unit<DT, VEC> q[kTokenBatch];
+  uint4* ring = reinterpret_cast<uint4*>(shared + 8 * 32 * VEC * 4) + warp * (kPieces * PieceRing<VEC>::kWords * 32) + lane;
+  auto by_cta = [&](int64_t begin, int64_t end, uint32_t key, int tile) {
+    const int u = tile * 32 + lane;
+    float acc[VEC] = {};
+    add_pieces<DT, VEC>(a, begin, end, u, warp, 8, ring, acc);
 #pragma unroll
-    for (int k = 0; k < kTokenBatch; ++k) {
-      const int64_t i = e + 8 * k < loose ? e + 8 * k : e;
-      token[k] = a.tokens[i < head ? begin + i : last * kChunk + (i - head)];
+    for (int i = 0; i < VEC; ++i) part[warp][i * 32 + lane] = acc[i];
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < 8; ++w)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += part[w][i * 32 + lane];
+      finish_run<DTO, VEC, ACC>(a, key, u, acc);
     }
-#pragma unroll
-    for (int k = 0; k < kTokenBatch; ++k)
-      if (e + 8 * k < loose && u < a.units)
-        q[k] = load_unit<DT, VEC>(a.grad, static_cast<int64_t>(token[k]) * a.grad_stride + static_cast<int64_t>(u) * VEC);
-#pragma unroll
-    for (int k = 0; k < kTokenBatch; ++k)
-      if (e + 8 * k < loose && u < a.units) add_unit<DT, VEC>(q[k], acc);
-  }
-  if (u < a.units) {
-    for (int64_t p = first + warp; p < last; p += 8 * 4) {
-      float f[4][VEC];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (p + 8 * k < last)
-          load_floats_plain<kDtF32, VEC>(a.chunk_sums, (p + 8 * k) * a.hidden + static_cast<int64_t>(u) * VEC, f[k]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (p + 8 * k < last)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] += f[k][i];
+    __syncthreads();
+  };
+  if (a.chunk_sums != nullptr) {
+    const int64_t n_items = static_cast<int64_t>(*a.n_long) * a.tiles;
+    const int together = n_items > 4 * static_cast<int64_t>(gridDim.x) ? 8 : 1;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * together; base < n_items; base += static_cast<int64_t>(gridDim.x) * together) {
+      if (together > 1) {
+        const int64_t mine = base + warp;
+        bool big = false;
+        if (mine < n_items) {
+          const uint2 run = a.long_runs[mine / a.tiles];
+          const int64_t begin = a.begins[run.y];
+          big = run.x - begin >= kWarpRun;
+          if (!big) {
+            const int u = static_cast<int>(mine % a.tiles) * 32 + lane;
+            float acc[VEC] = {};
+            add_pieces<DT, VEC>(a, begin, run.x, u, 0, 1, ring, acc);
+            finish_run<DTO, VEC, ACC>(a, run.y, u, acc);
+          }
+        }
+        if (!__syncthreads_or(big)) continue;
+      }
+      for (int64_t item = base; item < base + together && item < n_items; ++item) {
+        const uint2 run = a.long_runs[item / a.tiles];
+        const int64_t begin = a.begins[run.y];
+        if (together == 1 || run.x - begin >= kWarpRun) by_cta(begin, run.x, run.y, static_cast<int>(item % a.tiles));
+      }
     }
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) part[warp][i * 32 + lane] = acc[i];
-  __syncthreads();
-  if (warp == 0 && u < a.units) {
-    for (int w = 1; w < 8; ++w)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += part[w][i * 32 + lane];
-    float old[VEC];
-    if constexpr (ACC) load_floats_plain<DTO, VEC>(a.out, static_cast<int64_t>(key) * a.hidden + static_cast<int64_t>(u) * VEC, old);
-    write_unit<DTO, VEC, ACC>(a, key, u, acc, old);
+  // no list: a long run holds a multiple of kLongRun, and the block of the first one takes it
+  const int64_t at = static_cast<int64_t>(blockIdx.x / a.tiles) * kLongRun;
+  const uint32_t key = a.keys[at];
+  if (key >= a.vocab || (at > 0 && a.keys[at - kLongRun] == key)) return;
+  int64_t begin = at;  // back to where the run begins, at most 63 positions
+  for (int k = 0; k < 2; ++k) {
+    const int64_t p = at - 1 - 32 * k - lane;
+    const unsigned other = ~__ballot_sync(0xFFFFFFFFu, p >= 0 && a.keys[p >= 0 ? p : 0] == key);
+    begin = at - 32 * k - (other ? __ffs(other) - 1 : 32);
+    if (other) break;
   }
-  __syncthreads();
+  if (begin + kLongRun <= a.n && a.keys[begin + kLongRun - 1] == key) by_cta(begin, run_end(a, begin), key, static_cast<int>(blockIdx.x % a.tiles));
 }
 
 // The runs that begin in a group of sorted positions show in the keys of the positions themselves and of the 63 behind
@@ -612,42 +713,10 @@ struct Stretch {
   }
 };
 
-// The blocks for the long runs.
-template <int DT, int DTO, int VEC, bool ACC>
-__device__ __forceinline__ void long_runs(const SumArgs& a, unsigned block, float (*part)[32 * VEC]) {
-  if (a.chunk_sums != nullptr) {
-    const int64_t n_items = static_cast<int64_t>(*a.n_long) * a.tiles;
-    for (int64_t item = block; item < n_items; item += a.long_blocks) {
-      const uint2 run = a.long_runs[item / a.tiles];
-      add_long_run<DT, DTO, VEC, ACC>(a, a.begins[run.y], run.x, run.y, static_cast<int>(item % a.tiles), part);
-    }
-    return;
-  }
-  // no list: a long run holds a multiple of kLongRun, and the block of the first one takes it
-  const int lane = threadIdx.x & 31;
-  const int64_t at = block / a.tiles * kLongRun;
-  const uint32_t key = a.keys[at];
-  if (key >= a.vocab || (at > 0 && a.keys[at - kLongRun] == key)) return;
-  int64_t begin = at;  // back to where the run begins, at most 63 positions
-  for (int k = 0; k < 2; ++k) {
-    const int64_t p = at - 1 - 32 * k - lane;
-    const unsigned other = ~__ballot_sync(0xFFFFFFFFu, p >= 0 && a.keys[p >= 0 ? p : 0] == key);
-    begin = at - 32 * k - (other ? __ffs(other) - 1 : 32);
-    if (other) break;
-  }
-  if (begin + kLongRun <= a.n && a.keys[begin + kLongRun - 1] == key)
-    add_long_run<DT, DTO, VEC, ACC>(a, begin, run_end(a, begin), key, static_cast<int>(block % a.tiles), part);
-}
-
-// The first long_blocks blocks: the long runs; zero.blocks of the others: rows without tokens.  In the rest a warp takes `group` sorted positions and a
-// tile of 32 V vectors and adds the runs that begin there, then the next such item: one stream of tokens, whatever
-// the runs' lengths and the items' borders.  Each lane brings its V vectors of the next 15 / V tokens (7 / V with ACC) into its own
-// slots of shared memory by asynchronous copies and reads back only what it copied itself, so nothing but the copies' own
-// completion is waited for.  With ACC the warp also brings what the table holds, for a run's last token.
-// The blocks behind those for the long runs: the ones that sum and the zero-filling ones take turns, as far as there are
+// The blocks of row_stream_kernel and its like: the ones that sum and the zero-filling ones take turns, as far as there are
 // both, so that they share the SMs.  Whether this is a zero-filling one; `block` becomes its index among its kind.
 __device__ __forceinline__ bool take_turns(const SumArgs& a, unsigned& block) {
-  const unsigned sums = gridDim.x - a.long_blocks - a.zero.blocks, both = sums < a.zero.blocks ? sums : a.zero.blocks;
+  const unsigned sums = gridDim.x - a.zero.blocks, both = sums < a.zero.blocks ? sums : a.zero.blocks;
   bool fill;
   if (block < 2 * both) {
     fill = block & 1u;
@@ -663,19 +732,23 @@ template <bool ACC, int V>
 struct Ring {
   static constexpr int kDepth = (ACC ? 8 : 16) / V;
 };
+// zero.blocks of the blocks: rows without tokens.  In the others a warp takes `group` sorted positions and a tile of 32 V
+// vectors and adds the runs that begin there, then the next such item: one stream of tokens, whatever the runs' lengths
+// and the items' borders.  Each lane brings its V vectors of the next 15 / V tokens (7 / V with ACC) into its own slots of
+// shared memory by asynchronous copies and reads back only what it copied itself, so nothing but the copies' own
+// completion is waited for.  With ACC the warp also brings what the table holds, for a run's last token.
 template <int DT, int DTO, bool ACC, int V>
 __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __grid_constant__ SumArgs a) {
+  follow_previous();
   constexpr int VEC = Elem<DT>::kPerVec, kOld = ACC ? VEC * Elem<DTO>::kBytes / 16 : 0, kSlot = V * (1 + kOld);  // 16-byte words
   extern __shared__ __align__(16) unsigned char shared[];
   unsigned block = blockIdx.x;
-  if (block < a.long_blocks) return long_runs<DT, DTO, VEC, ACC>(a, block, reinterpret_cast<float(*)[32 * VEC]>(shared));
-  block -= a.long_blocks;
   if (take_turns(a, block)) return fill_rows(a.zero, block);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* ring = reinterpret_cast<uint4*>(shared) + warp * (Ring<ACC, V>::kDepth * kSlot * 32) + lane;  // [slot][word][lane]
   const int row_tiles = (a.units + 32 * V - 1) / (32 * V);
   const int64_t n_items = (a.n + a.group - 1) / a.group * row_tiles;
-  const int64_t stride = static_cast<int64_t>(gridDim.x - a.zero.blocks - a.long_blocks) * 8;
+  const int64_t stride = static_cast<int64_t>(gridDim.x - a.zero.blocks) * 8;
 
   int64_t item = static_cast<int64_t>(block) * 8 + warp;  // the next one to be opened; its window is on the way
   Window ahead, now;
@@ -761,44 +834,49 @@ __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __gr
   }
 }
 
-// The same for rows that are not whole, aligned vectors: element by element, a few tokens' loads in flight together.
+// The same for rows that are not whole, aligned vectors: kAny elements per lane, a few tokens' loads in flight together.
+constexpr int kAny = 4;
 template <int DT, int DTO, bool ACC>
-__global__ void __launch_bounds__(256) row_sums_any_kernel(const __grid_constant__ SumArgs a) {
-  extern __shared__ __align__(16) unsigned char shared[];
+__global__ void __launch_bounds__(256, 3) row_sums_any_kernel(const __grid_constant__ SumArgs a) {
+  follow_previous();
   unsigned block = blockIdx.x;
-  if (block < a.long_blocks) return long_runs<DT, DTO, 1, ACC>(a, block, reinterpret_cast<float(*)[32]>(shared));
-  block -= a.long_blocks;
   if (take_turns(a, block)) return fill_rows(a.zero, block);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n_items = (a.n + a.group - 1) / a.group * a.tiles;
-  const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.zero.blocks - a.long_blocks) * 8;
+  const int row_tiles = (a.units + 32 * kAny - 1) / (32 * kAny);
+  const int64_t n_items = (a.n + a.group - 1) / a.group * row_tiles;
+  const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.zero.blocks) * 8;
   for (int64_t item = static_cast<int64_t>(block) * 8 + warp; item < n_items; item += n_warps) {
-    const int64_t group = item / a.tiles;
-    const int u = static_cast<int>(item - group * a.tiles) * 32 + lane;
+    const int64_t group = item / row_tiles;
+    const int u0 = static_cast<int>(item - group * row_tiles) * (32 * kAny) + lane;
     Window w;
     Stretch s;
     w.load(a, group * a.group);
     s.find(a, w);
-    float acc[1] = {};
+    float acc[kAny][1] = {};
     for (int t0 = s.from; t0 < s.to; t0 += kTokenBatch) {
-      Unit<DT, 1> q[kTokenBatch];
+      Unit<DT, 1> q[kTokenBatch][kAny];
 #pragma unroll
       for (int t = 0; t < kTokenBatch; ++t) {
         const int64_t at = static_cast<int64_t>(w.token_at(t0 + t < s.to ? t0 + t : t0)) * a.grad_stride;
-        if (u < a.units) q[t] = load_unit<DT, 1>(a.grad, at + u);
+#pragma unroll
+        for (int j = 0; j < kAny; ++j)
+          if (u0 + 32 * j < a.units) q[t][j] = load_unit<DT, 1>(a.grad, at + u0 + 32 * j);
       }
 #pragma unroll
       for (int t = 0; t < kTokenBatch; ++t) {
         if (t0 + t >= s.to) break;
-        const uint32_t row = w.key_at(t0 + t);
+        const int64_t row = w.key_at(t0 + t);
         const bool end = s.last_of_run(t0 + t);
-        if (u >= a.units) continue;
-        add_unit<DT, 1>(q[t], acc);
-        if (!end) continue;
-        float old[1] = {};
-        if constexpr (ACC) load_floats_plain<DTO, 1>(a.out, static_cast<int64_t>(row) * a.hidden + u, old);
-        write_unit<DTO, 1, ACC>(a, row, u, acc, old);
-        acc[0] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kAny; ++j) {
+          if (u0 + 32 * j >= a.units) continue;
+          add_unit<DT, 1>(q[t][j], acc[j]);
+          if (!end) continue;
+          float old[1] = {};
+          if constexpr (ACC) load_floats_plain<DTO, 1>(a.out, row * a.hidden + u0 + 32 * j, old);
+          write_unit<DTO, 1, ACC>(a, row, u0 + 32 * j, acc[j], old);
+          acc[j][0] = 0.0f;
+        }
       }
     }
   }
@@ -893,8 +971,8 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, 
       if (e != cudaSuccess) return e;
     }
     s.zero = share_of(rest, p + 1 < passes ? a.vocab / passes : a.vocab);
-    sort_move_kernel<<<s.sort_blocks + s.zero.blocks, kSortThreads, 0, stream>>>(s);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_dependent(true, sort_move_kernel, s.sort_blocks + s.zero.blocks, kSortThreads, 0, stream, s);
     if (e != cudaSuccess) return e;
   }
   *where = (passes - 1) & 1;
@@ -922,16 +1000,26 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
   // Up to 1024 tokens a CTA adds even the longest run while the others are added (at most 16 batches of loads per warp);
   // beyond, the launch for the chunks pays (3001 skewed tokens of 1000 columns: 58 us without, 41 with it).
   const bool chunks = a.n_ids > 1024;
+  const bool few = a.n_ids <= kRankMax;  // short kernels one behind the other: their launches overlap
   if (chunks) {
     s.chunk_sums = w.chunk_sums;
-    const int64_t items = a.n_ids / kChunk * s.tiles;
+    constexpr int kUnits = VEC > 1 ? 1 : kAny;
+    const int64_t items = a.n_ids / kChunk * ((s.units + 32 * kUnits - 1) / (32 * kUnits));
     const int64_t grid = (items + 7) / 8 < sms * 5 ? (items + 7) / 8 : sms * 5;
     s.zero = share_of(rest, (rest.end - rest.begin) / 2);
-    chunk_sums_kernel<DT, VEC><<<static_cast<unsigned>(grid) + s.zero.blocks, 256, 0, stream>>>(s);
+    const cudaError_t e = launch_dependent(few, chunk_sums_kernel<DT, VEC, kUnits>, static_cast<unsigned>(grid) + s.zero.blocks, 256, 0, stream, s);
+    if (e != cudaSuccess) return e;
   }
   s.zero = share_of(rest, rest.end - rest.begin);
-  const int64_t max_long = a.n_ids / kLongRun * s.tiles;
-  s.long_blocks = static_cast<unsigned>(!chunks ? (a.n_ids + kLongRun - 1) / kLongRun * s.tiles : max_long < 2 * sms ? max_long : 2 * sms);
+  if (a.n_ids >= kLongRun) {
+    // with a list three CTAs per SM share it out
+    constexpr size_t smem = size_t(8) * 32 * VEC * 4 + size_t(8) * kPieces * PieceRing<VEC>::kWords * 32 * 16;
+    cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(long_runs_kernel<DT, DTO, VEC, ACC>), 256, smem, -1, nullptr);
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = chunks ? a.n_ids / kLongRun * s.tiles : (a.n_ids + kLongRun - 1) / kLongRun * s.tiles;
+    e = launch_dependent(few, long_runs_kernel<DT, DTO, VEC, ACC>, static_cast<unsigned>(chunks && blocks > 3 * sms ? 3 * sms : blocks), 256, smem, stream, s);
+    if (e != cudaSuccess) return e;
+  }
   const auto finish = [&](auto kern, int vectors, size_t smem) {
     int per_sm = 4;
     const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), 256, smem, -1, &per_sm);
@@ -942,8 +1030,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * tiles < sms * per_sm * 8 * 4) s.group /= 2;
     const int64_t items = (a.n_ids + s.group - 1) / s.group * tiles;
     const int64_t token_blocks = (items + 7) / 8 < sms * per_sm ? (items + 7) / 8 : sms * per_sm;
-    kern<<<static_cast<unsigned>(s.long_blocks + token_blocks) + s.zero.blocks, 256, smem, stream>>>(s);
-    return cudaGetLastError();
+    return launch_dependent(few, kern, static_cast<unsigned>(token_blocks) + s.zero.blocks, 256, smem, stream, s);
   };
   if constexpr (VEC > 1) {
     // Several vectors per lane share what a token costs in instructions (1 -> 4 vectors: 120 -> 95 us for the sums of
@@ -958,7 +1045,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     if (enough(2, 8)) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
     return finish(row_stream_kernel<DT, DTO, ACC, 1>, 1, kSmem);
   } else {
-    return finish(row_sums_any_kernel<DT, DTO, ACC>, 1, 8 * 32 * 4);
+    return finish(row_sums_any_kernel<DT, DTO, ACC>, kAny, 0);
   }
 }
 

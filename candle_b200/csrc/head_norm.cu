@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kThreads) forward_any_kernel(const ForwardArgs
 // A warp keeps the weights' gradient of its rows in its own line of `partials` (each lane its own columns).
 template <int DT, int DTC>
 __global__ void __launch_bounds__(kThreads) backward_any_kernel(const BackwardArgs a) {
+  follow_previous();
   const Common& c = a.c;
   const int lane = threadIdx.x & 31;
   const int half = c.rotary / 2, items = c.dim - half;
@@ -459,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, NI == 2 ? 2 : 3) forward_kernel(cons
 template <int DT, int DTC, int PV, int NI, int R, bool INTER>
 __global__ void __launch_bounds__(kThreads, NI == 2 ? 1 : 2) backward_kernel(const BackwardArgs a, const Walk q_walk,
                                                                                   const Walk k_walk) {
+  follow_previous();
   extern __shared__ float line[];  // [warp][dim]
   const Common& c = a.c;
   constexpr int kBytes = Elem<DT>::kBytes, kWords = Vec<DT, PV>::kWords, P2 = PV / 2;

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(kThreads) alpha_partials_kernel(const RmsBackw
 
 template <int DT>
 __global__ void __launch_bounds__(kThreads) dx_kernel(const RmsBackwardArgs a, const float2* factors) {
+  follow_previous();
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float2 f = factors[row];
     for (int c = threadIdx.x; c < a.n; c += kThreads) {
@@ -85,6 +86,7 @@ constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(kSumWarps * 32) sum_partials_kernel(const float* partials, int n_partials, int cols,
                                                                       float* out, int split, float* out2) {
   __shared__ float part[kSumWarps][33];
+  follow_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float acc = 0.0f;
@@ -216,6 +218,7 @@ __device__ __forceinline__ void add_groups(const float* line, int groups, int n,
 
 template <int DT, int VB, int U, bool SUM, int T>
 __global__ void __launch_bounds__(T, 512 / T) rows_kernel(const FastArgs f) {
+  follow_previous();
   extern __shared__ __align__(16) unsigned char shared[];
   using V = typename VecOf<VB>::type;
   constexpr int P2 = VB / Elem<DT>::kBytes / 2, kInputs = SUM ? 3 : 2, kStages = Ring<U>::kStages, VPT = U * 16 / VB;
@@ -343,6 +346,7 @@ __device__ __forceinline__ void bring_rows(unsigned char* to, const void* from, 
 
 template <int DT, int E, bool SUM>
 __global__ void __launch_bounds__(kThreads, 2) rows_any_kernel(const FastArgs f) {
+  follow_previous();
   extern __shared__ __align__(16) unsigned char shared[];
   constexpr int kInputs = SUM ? 3 : 2, kBytes = Elem<DT>::kBytes;
   const RmsBackwardArgs& a = f.a;
@@ -510,8 +514,8 @@ cudaError_t launch_dt(const RmsBackwardArgs& a, float* partials, float2* factors
 
 cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols, float* out, int split, float* out2,
                                 cudaStream_t stream) {
-  sum_partials_kernel<<<(cols + 31) / 32, kSumWarps * 32, 0, stream>>>(partials, n_partials, cols, out, split, out2);
-  return cudaGetLastError();
+  return launch_dependent(true, sum_partials_kernel, static_cast<unsigned>((cols + 31) / 32), kSumWarps * 32, 0, stream, partials, n_partials,
+                          cols, out, split, out2);
 }
 
 int64_t rms_backward_workspace(int64_t rows, int n) {
