@@ -706,6 +706,10 @@ cudaError_t launch_forward_vec(const ForwardArgs& a, const Walk& w, int64_t grid
   return cudaGetLastError();
 }
 
+// Rows per lane and unit: 32 bytes of each vector's elements, however narrow the vectors.
+template <int DT, int PV>
+constexpr int kUnitRows = 2 * Elem<DT>::kPerVec / PV;
+
 template <int DT, int DTC, int PV>
 cudaError_t launch_forward_pv(const ForwardArgs& a, cudaStream_t stream, bool* done) {
   const Common& c = a.c;
@@ -718,8 +722,9 @@ cudaError_t launch_forward_pv(const ForwardArgs& a, cudaStream_t stream, bool* d
     const Walk w = plan_walk(c, c.q_heads, c.k_heads, items, 1, cap, grid);
     return launch_forward_vec<DT, DTC, PV, 2, 1>(a, w, grid, stream);
   }
-  Walk w = plan_walk(c, c.q_heads, c.k_heads, items, 2, cap, grid);
-  if (w.n_units >= 2 * cap * kWarps) return launch_forward_vec<DT, DTC, PV, 1, 2>(a, w, grid, stream);
+  constexpr int kRows = kUnitRows<DT, PV>;
+  Walk w = plan_walk(c, c.q_heads, c.k_heads, items, kRows, cap, grid);
+  if (w.n_units >= 2 * cap * kWarps) return launch_forward_vec<DT, DTC, PV, 1, kRows>(a, w, grid, stream);
   grid = 0;
   w = plan_walk(c, c.q_heads, c.k_heads, items, 1, cap, grid);
   return launch_forward_vec<DT, DTC, PV, 1, 1>(a, w, grid, stream);
@@ -770,7 +775,7 @@ cudaError_t launch_backward_pv(BackwardArgs& a, cudaStream_t stream, bool* done)
   *done = items <= 64;
   if (!*done) return cudaSuccess;
   if (items > 32) return launch_backward_vec<DT, DTC, PV, 2, 1>(a, items, 1, stream);
-  return launch_backward_vec<DT, DTC, PV, 1, 2>(a, items, 2, stream);
+  return launch_backward_vec<DT, DTC, PV, 1, kUnitRows<DT, PV>>(a, items, 2, stream);
 }
 
 template <int DT, int DTC>
