@@ -270,6 +270,31 @@ def test_table_grad_of_whole_numbers_is_exact(cb, n, vocab, hidden, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,vocab,hidden,kind", [
+    (1024, 50, 72, "skew"), (1025, 50, 72, "skew"), (8192, 90, 72, "skew"), (8193, 90, 72, "skew"),  # where the launches change
+    (9000, 262145, 24, "uniform"), (20000, (1 << 27) + 3, 1, "skew"),  # three and four digits
+    (40000, 300, 4096, "uniform"), (40000, 300, 4096, "skew"), (60000, 200, 2056, "skew"),  # many long runs, several vectors per lane
+    (30000, 30000, 4096, "uniform"), (9000, 9, 515, "falling"),
+])
+def test_table_grad_over_the_kernels_of_larger_batches(cb, n, vocab, hidden, kind):
+    # whole numbers of at most 8: exact, as above
+    g = torch.Generator(device="cuda").manual_seed(n)
+    grad = torch.randint(-8, 9, (n, hidden), generator=g, device="cuda", dtype=torch.int32)
+    ids = make_ids(n + 1, n, vocab, kind)
+    for dtype, wide in ((torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, True)):
+        if not wide and vocab * hidden > 1 << 27:
+            continue
+        out_dtype = torch.float32 if wide else dtype
+        got = cb.embedding_backward(grad.to(dtype), ids, vocab, out_dtype=out_dtype)
+        want = torch.zeros(vocab, hidden, dtype=torch.float32, device="cuda").index_add_(0, ids, grad.float())
+        assert torch.equal(got, want.to(out_dtype))
+        acc = torch.full((vocab, hidden), 2.0, dtype=out_dtype, device="cuda")
+        cb.embedding_backward(grad.to(dtype), ids, vocab, scale=0.5, out=acc, accumulate=True)
+        assert torch.equal(acc, (2.0 + 0.5 * want).to(out_dtype))
+        del got, want, acc
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("n,vocab,hidden,kind,id_dtype", [(1, 100, 64, "uniform", torch.int64), (513, 100, 1000, "skew", torch.uint32),
@@ -354,7 +379,7 @@ def norm_grad_64(grad, x, w, eps):
     return dx, size, terms.sum(0), terms.abs().sum(0)
 
 
-NORM_SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 128), (300, 96), (1000, 768), (33, 1000), (64, 2048), (9, 4096), (700, 4096), (1200, 8192),
+NORM_SHAPES = [(600, 3348), (50, 6150), (7, 12000), (400, 4097), (333, 130), (1, 1), (1, 8), (3, 7), (5, 64), (2, 128), (300, 96), (1000, 768), (33, 1000), (64, 2048), (9, 4096), (700, 4096), (1200, 8192),
                (2, 8192), (5, 10000), (3, 16384), (40, 257), (20000, 64)]
 
 
