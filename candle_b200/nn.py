@@ -20,13 +20,22 @@ class Embedding:
     def hidden_size(self) -> int:
         return self._hidden_size
 
-    def forward(self, indexes: torch.Tensor, *, check: bool = True) -> torch.Tensor:
-        # candle-nn/src/embedding.rs:29-36
+    def forward(self, indexes: torch.Tensor, *, scale: float | None = None, check: bool = True) -> torch.Tensor:
+        # candle-nn/src/embedding.rs:29-36; with `scale` the multiplication that some models put behind it, in the same launch
+        if scale is not None:
+            return ops.embedding_scaled(self._embeddings, indexes, scale, check=check)
         final_dims = list(indexes.shape) + [self._hidden_size]
         values = ops.index_select(self._embeddings, indexes.reshape(-1), 0, check=check)
         return values.reshape(final_dims)
 
     __call__ = forward
+
+    def backward(self, grad: torch.Tensor, indexes: torch.Tensor, *, scale: float = 1.0, out: torch.Tensor | None = None,
+                 accumulate: bool = False, out_dtype: torch.dtype | None = None, padding_id: int | None = None,
+                 check: bool = True) -> torch.Tensor:
+        """Gradient of ``forward(indexes, scale=scale)`` with respect to the table (``ops.embedding_backward``)."""
+        return ops.embedding_backward(grad, indexes, self._embeddings.shape[0], scale=scale, out=out, accumulate=accumulate,
+                                      out_dtype=out_dtype, padding_id=padding_id, check=check)
 
 
 class LayerNorm:
@@ -86,6 +95,11 @@ class RmsNorm:
         return self._inner.forward(xs, residual=residual)
 
     __call__ = forward
+
+    def backward(self, grad: torch.Tensor, xs: torch.Tensor, *, grad_sum: torch.Tensor | None = None):
+        """``(dxs, dweight)`` for the gradient of ``forward(xs)`` (``ops.rms_norm_backward``; after a forward with a residual
+        pass the sum as ``xs``)."""
+        return ops.rms_norm_backward(grad, xs, self._inner.weight(), self._inner.eps, grad_sum=grad_sum)
 
 
 class QEmbedding:

@@ -11,6 +11,8 @@
  *   index_select(t, ids, dim)                Tensor::index_select            tensor.rs:1568-1589
  *   Embedding{table, hidden}.forward(ids)    candle_nn::Embedding::forward   embedding.rs:28-37
  *   QTensor::embedding / embedding_rms_norm  (new: lookups out of GGML blocks)
+ *   ops::embedding_scaled, embedding_backward, rms_norm_backward, qk_norm_rope, qk_norm_rope_backward
+ *                                            (new: training and serving operators beside the path)
  *
  * A Tensor here is a non-owning view of caller-allocated device memory (pointer, dims, dtype) --
  * the library never allocates -- and every function takes the destination view and a stream.
@@ -308,6 +310,99 @@ class Embedding {
   Tensor embeddings_;
   int64_t hidden_size_;
 };
+
+/* Training and serving operators beside the path (no counterpart in candle; see candle_b200.h for the formulas). */
+namespace ops {
+
+/* Scratch device memory; *_workspace says how many bytes a call needs. */
+struct Workspace {
+  void* data = nullptr;
+  int64_t bytes = 0;
+};
+
+/* out = scale * table[ids], rounded once; ids of any shape. */
+inline void embedding_scaled(const Tensor& table, const Tensor& ids, float scale, Tensor& out, cb200_status* status,
+                             cb200_stream_t stream) {
+  if (table.rank() != 2 || !table.contiguous) throw Error("index-select requires contiguous tensors");
+  if (!is_float(table.dtype)) throw Error(std::string("unsupported dtype ") + dtype_name(table.dtype) + " for embedding");
+  if (!ids.contiguous) throw Error("index-select ids must be contiguous on the device");
+  Shape want = ids.dims;
+  want.push_back(table.dims[1]);
+  detail::check_out(out, want, table.dtype, "embedding");
+  detail::check_rc(cb200_embedding_scaled(table.data, ids.data, out.data, table.dims[0], static_cast<int32_t>(table.dims[1]),
+                                          ids.elem_count(), scale, static_cast<int>(table.dtype), detail::id_code(ids.dtype),
+                                          status, stream));
+}
+
+inline int64_t embedding_backward_workspace(int64_t vocab, int64_t hidden, int64_t n_ids) {
+  int64_t bytes = 0;
+  detail::check_rc(cb200_embedding_backward_workspace(vocab, static_cast<int32_t>(hidden), n_ids, &bytes));
+  return bytes;
+}
+
+/* out[v] = scale * sum of the rows of grad whose id is v, or with `accumulate` added to out; grad is ids.dims ++ [hidden], out
+ * [vocab, hidden] of grad's type or F32; tokens of `padding_id` (-1: none) contribute nothing. */
+inline void embedding_backward(const Tensor& grad, const Tensor& ids, Tensor& out, Workspace workspace, cb200_status* status,
+                               cb200_stream_t stream, float scale = 1.0f, bool accumulate = false, int64_t padding_id = -1) {
+  if (!is_float(grad.dtype)) throw Error(std::string("unsupported dtype ") + dtype_name(grad.dtype) + " for embedding-backward");
+  if (!grad.contiguous || !ids.contiguous) throw Error("embedding-backward requires contiguous tensors");
+  Shape want = ids.dims;
+  if (grad.rank() == 0 || out.rank() != 2) throw Error("unexpected rank in embedding-backward " + dims_string(grad.dims) + " " + dims_string(out.dims));
+  want.push_back(grad.dims.back());
+  if (grad.dims != want) throw Error("shape mismatch in embedding-backward " + dims_string(grad.dims) + " " + dims_string(ids.dims));
+  detail::check_out(out, {out.dims[0], grad.dims.back()}, out.dtype == DType::F32 ? DType::F32 : grad.dtype, "embedding-backward");
+  detail::check_rc(cb200_embedding_backward(grad.data, grad.dims.back(), ids.data, out.data, out.dims[0],
+                                            static_cast<int32_t>(grad.dims.back()), ids.elem_count(), scale, padding_id,
+                                            accumulate ? 1 : 0, static_cast<int>(grad.dtype), static_cast<int>(out.dtype),
+                                            detail::id_code(ids.dtype), workspace.data, workspace.bytes, status, stream));
+}
+
+inline int64_t rms_norm_backward_workspace(int64_t rows, int64_t cols) {
+  int64_t bytes = 0;
+  detail::check_rc(cb200_rms_norm_backward_workspace(rows, static_cast<int32_t>(cols), &bytes));
+  return bytes;
+}
+
+/* dxs and dalpha (F32) of rms_norm(xs, alpha, eps) for the gradient `grad` of its result; `grad_sum` is added to dxs. */
+inline void rms_norm_backward(const Tensor& grad, const Tensor& xs, const Tensor& alpha, float eps, Tensor& dxs, Tensor& dalpha,
+                              Workspace workspace, cb200_stream_t stream, const Tensor* grad_sum = nullptr) {
+  if (xs.rank() == 0) throw Error("unexpected rank, expected: at least 1, got: 0");
+  if (alpha.rank() != 1 || xs.dims.back() != alpha.dims[0])
+    throw Error("shape mismatch in rms-norm " + dims_string(xs.dims) + " " + dims_string(alpha.dims));
+  const Tensor* params[] = {&alpha};
+  const char* names[] = {"alpha"};
+  detail::norm_checks(xs, params, names, 1, nullptr);
+  for (const Tensor* g : {&grad, grad_sum})
+    if (g != nullptr && (g->dims != xs.dims || g->dtype != xs.dtype || !g->contiguous))
+      throw Error("shape mismatch in rms-norm-backward, xs: " + dims_string(xs.dims) + ", gradient: " + dims_string(g->dims));
+  detail::check_out(dxs, xs.dims, xs.dtype, "rms-norm-backward");
+  detail::check_out(dalpha, alpha.dims, DType::F32, "rms-norm-backward");
+  const int64_t cols = xs.dims.back(), rows = cols ? xs.elem_count() / cols : 0;
+  detail::check_rc(cb200_rms_norm_backward(grad.data, xs.data, alpha.data, grad_sum ? grad_sum->data : nullptr, dxs.data,
+                                           dalpha.data, rows, static_cast<int32_t>(cols), eps, static_cast<int>(xs.dtype),
+                                           workspace.data, workspace.bytes, stream));
+}
+
+/* Head norms with rotation and their gradient, on views of any strides: `args` and the views are those of the C ABI. */
+inline void qk_norm_rope(const cb200_heads& q, const cb200_heads& k, const cb200_heads& q_out, const cb200_heads& k_out,
+                         const cb200_qk_args& args, cb200_status* status, cb200_stream_t stream) {
+  detail::check_rc(cb200_qk_norm_rope(&q, &k, &q_out, &k_out, &args, status, stream));
+}
+inline int64_t qk_norm_rope_backward_workspace(int64_t dim) {
+  int64_t bytes = 0;
+  detail::check_rc(cb200_qk_norm_rope_backward_workspace(static_cast<int32_t>(dim), &bytes));
+  return bytes;
+}
+inline void qk_norm_rope_backward(const cb200_heads& grad_q, const cb200_heads& grad_k, const cb200_heads& q, const cb200_heads& k,
+                                  const cb200_heads& dq, const cb200_heads& dk, Tensor& dq_weight, Tensor& dk_weight,
+                                  const cb200_qk_args& args, Workspace workspace, cb200_status* status, cb200_stream_t stream) {
+  detail::check_out(dq_weight, {args.dim}, DType::F32, "qk-norm-rope-backward");
+  detail::check_out(dk_weight, {args.dim}, DType::F32, "qk-norm-rope-backward");
+  detail::check_rc(cb200_qk_norm_rope_backward(&grad_q, &grad_k, &q, &k, &dq, &dk, dq_weight.data, dk_weight.data, &args,
+                                               workspace.data, workspace.bytes, status, stream));
+}
+
+}  // namespace ops
 
 /* Raw GGML blocks + logical shape on the device (candle-core/src/quantized/mod.rs:35-38). */
 struct QTensor {

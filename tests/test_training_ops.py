@@ -187,6 +187,40 @@ def test_c_entry_points_refuse_on_the_host():
         assert lib.cb200_qk_norm_rope_backward(*args) < 0, i
 
 
+def test_cpp_mirror_compiles_and_refuses(tmp_path):
+    import os
+    import shutil
+    import subprocess
+
+    import candle_b200  # noqa: F401  (makes sure the library is built)
+
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib_dir, exe = os.path.join(root, "candle_b200", "_lib"), str(tmp_path / "training_checks")
+    subprocess.run([gxx, "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(root, "include"), "-o", exe,
+                    os.path.join(root, "tests", "cpp", "training_checks.cpp"), "-L", lib_dir, "-l:libcandle_b200.so",
+                    f"-Wl,-rpath,{lib_dir}"], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    lines = out.stdout.strip().splitlines()
+    assert out.returncode == 0 and len(lines) == 11 and all(line.startswith("ok ") for line in lines), out.stdout + out.stderr
+
+
+def test_modules_pass_their_arguments_on(monkeypatch):
+    from candle_b200 import nn, ops
+
+    seen = []
+    monkeypatch.setattr(ops, "embedding_scaled", lambda *a, **k: seen.append(("scaled", a[2], k)))
+    monkeypatch.setattr(ops, "embedding_backward", lambda *a, **k: seen.append(("backward", a[2], k["scale"])))
+    monkeypatch.setattr(ops, "rms_norm_backward", lambda *a, **k: seen.append(("norm", a[3], k["grad_sum"])))
+    e, n, ids = nn.Embedding(torch.zeros(10, 8), 8), nn.RmsNorm(torch.ones(8), 1e-5), torch.zeros(3, dtype=torch.int64)
+    e.forward(ids, scale=2.0, check=False)
+    e.backward(torch.zeros(3, 8), ids, scale=2.0)
+    n.backward(torch.zeros(3, 8), torch.zeros(3, 8))
+    assert seen == [("scaled", 2.0, {"check": False}), ("backward", 10, 2.0), ("norm", 1e-5, None)]
+
+
 # ---- scaled lookup -----------------------------------------------------------------------------------------
 
 
@@ -721,30 +755,34 @@ def block_inputs(dtype, seed, b=3, t=37):
     return p, ids, g
 
 
-@pytest.mark.gpu
-def test_operators_together_against_64_bits(cb):
-    p, ids, g = block_inputs(torch.float32, 100)
-    got = block_step(cb, p, ids, g)
+def rel_to_formulas(p, ids, g, got):
+    """How far block_step's results are from the formulas' in 64 bits: the largest relative error in norm."""
+    hidden, d = p["table"].shape[1], p["wq"].shape[0]
     P = {n: t.double().requires_grad_(n not in ("cos", "sin")) for n, t in p.items()}
-    e = P["table"][ids] * math.sqrt(256)
+    e = P["table"][ids] * math.sqrt(hidden)
     h = e + P["res"]
     y = h * (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * P["alpha"]
-    qkv = (y @ P["proj"]).view(3, 37, 6, 64)
+    qkv = (y @ P["proj"]).view(*ids.shape, 6, d)
     c, s = P["cos"][None, :, None], P["sin"][None, :, None]
 
     def head(x, w):
         u = x * (x.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * w
-        a, b = u[..., :32], u[..., 32:]
+        a, b = u[..., :d // 2], u[..., d // 2:]
         return torch.cat([a * c - b * s, a * s + b * c], -1)
 
     oq, ok = head(qkv[..., :4, :], P["wq"]), head(qkv[..., 4:, :], P["wk"])
     loss = (oq * g[0].double()).sum() + (ok * g[1].double()).sum() + (h * g[2].double()).sum()
     loss.backward()
     want = (oq, ok, h, P["wq"].grad, P["wk"].grad, P["proj"].grad, P["alpha"].grad, P["res"].grad, P["table"].grad)
+    return max(((a.double() - b).norm() / b.norm()).item() for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_operators_together_against_64_bits(cb):
+    p, ids, g = block_inputs(torch.float32, 100)
     # f32 throughout; the products (torch's, possibly with fewer bits) have 256 and 384 terms of size 1/16: in norm, errors
     # of a few hundred U of the terms, which are at most sqrt(384) times the result's size
-    for a, b in zip(got, want):
-        assert (a.double() - b).norm() <= 400 * math.sqrt(384) * U * b.norm()
+    assert rel_to_formulas(p, ids, g, block_step(cb, p, ids, g)) <= 400 * math.sqrt(384) * U
 
 
 @pytest.mark.gpu
