@@ -2,7 +2,14 @@
 //   forward   u = x r w,  r = 1 / sqrt(mean(x^2) + eps);   out = R u   (R: the rotation of the token's position)
 //   gradient  v = R^T g;  dx = r (v w - x r^2 mean(v w x));  dw = sum over rows of v x r
 // A row is one head of one token.  As separate operators (norm, rotation) queries and keys make two trips through
-// memory and are rounded twice; here one.
+// memory and are rounded twice; here one.  Everything is f32 inside, rounded once to T when it is stored; the sums of the
+// weights' gradients stay in f32.
+//
+// Measured (B200, 32 + 8 heads of 128 columns, bf16): forward, 16384 tokens, 336 MB: 61 us, 5.5 TB/s, 0.85 of a copy's rate
+// (the same kernel with scalar arithmetic and IEEE divisions: 72 us, bound by issue slots at 22 instructions per
+// element); gradient, 16384 tokens, 504 MB: 97 us, 5.2 TB/s with the sum of the partial gradients (with v computed twice
+// instead of kept 106 us; rows staged through shared memory instead of registers 104 us).  64 tokens: 2.6 us on the
+// device, a launch's latency.
 #include "launch.h"
 
 namespace cb200 {
@@ -328,6 +335,7 @@ struct Place {
 };
 
 // A unit's rows share token and weight, so weight and angle are multiplied once per unit: with half-split pairs
+// (r: a row's inverse root mean square, by the approximate reciprocal square root, off by at most 2 ulp)
 //   y1 = (x1 r) (w1 cos) - (x2 r) (w2 sin),   y2 = (x1 r) (w1 sin) + (x2 r) (w2 cos).
 template <int DT, int DTC, int PV, int NI, int R, bool INTER>
 __global__ void __launch_bounds__(kThreads, NI == 2 ? 2 : 3) forward_kernel(const ForwardArgs a, const Walk walk) {

@@ -1,7 +1,10 @@
 // Gradient of the RMS norm.  With r = 1 / sqrt(mean(x^2) + eps) of a row and s = mean(g * alpha * x):
 //   dx = r * (g * alpha - x * r^2 * s) + grad_sum        dalpha = sum over rows of g * x * r
 // A row needs two sums (x^2 and g * alpha * x) before its dx can be written; dalpha is a sum over rows, held in
-// f32 per block of rows and added up by a second kernel in a fixed order.
+// f32 per block of rows and added up by a second kernel in a fixed order.  f32 inside, dx rounded once.
+//
+// Bound by memory: 65536 x 8192 bf16 with grad_sum (4.3 GB) 640 us, 6.7 TB/s, a little above a plain copy's rate (three
+// reads per write); 32768 x 8192 f32 (3.2 GB) 534 us; 1000000 x 256 bf16 with grad_sum (2.0 GB) 325 us.
 #include "launch.h"
 
 namespace cb200 {

@@ -6,7 +6,7 @@
  * Conventions, identical for every function:
  *   - all tensor pointers are DEVICE pointers to contiguous row-major data whose start offset
  *     has already been applied by the caller (candle-nn/src/ops.rs:536-543 does the same
- *     `slice(o1..o2)` before launching); strides are never passed;
+ *     `slice(o1..o2)` before launching); strides are passed only where a call has arguments for them;
  *   - the CALLER allocates every output (candle: `unsafe { dev.alloc::<T>(el) }`,
  *     candle-nn/src/ops.rs:557); the library allocates and frees nothing and writes every
  *     output element of a call that succeeds;
