@@ -837,6 +837,7 @@ __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __gr
         for (int i = 0; i < VEC; ++i) acc[k][i] = 0.0f;
       }
     }
+    if constexpr (ACC) __syncwarp();  // the slot's next copies are not the reading lanes' own
   }
 }
 
