@@ -693,6 +693,8 @@ int cb200_embedding_backward(const void* grad, int64_t grad_stride, const void* 
   if (rc != CB200_OK) return rc;
   if (!valid_id_dtype(id_dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported ids dtype code %d", name, id_dtype);
   if (grad_stride < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative row stride", name);
+  if (padding_id < -1 || (padding_id >= vocab && padding_id != -1))
+    return fail(CB200_E_INVALID_ARGUMENT, "%s: the padding id %lld is no row of the table", name, (long long)padding_id);
   if (hidden > 0 && ((n_ids > 0 && (grad == nullptr || ids == nullptr)) || (vocab > 0 && out == nullptr)))
     return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
   if (n_ids > 0 && hidden > 0) {

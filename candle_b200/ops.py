@@ -551,7 +551,8 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
 
     ``grad`` is ``[*ids.shape, hidden]`` (rows may be strided).  The result is a fresh tensor of ``out_dtype``
     (``grad``'s, or f32) or ``out``; every row is written, zeros where no id points.  With ``accumulate`` the sums are
-    added to ``out`` and the other rows are not touched.  Tokens whose id is ``padding_id`` contribute nothing."""
+    added to ``out`` and the other rows are not touched.  Tokens whose id is ``padding_id``, a row
+    of the table, contribute nothing."""
     if grad.dtype not in _DTYPES:
         raise CandleError(f"unsupported dtype {grad.dtype} for embedding-backward")
     if grad.dim() == 0 or list(grad.shape[:-1]) != list(ids.shape):
@@ -568,6 +569,8 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     vocab = int(vocab)
     if vocab < 0:
         raise CandleError(f"the table of embedding-backward has {vocab} rows")
+    if padding_id is not None and not 0 <= padding_id < vocab:
+        raise CandleError(f"padding_id {padding_id} is no row of the table of embedding-backward, which has {vocab} rows")
     if out_dtype is None:
         out_dtype = grad.dtype if out is None else out.dtype
     if out_dtype != grad.dtype and out_dtype != torch.float32:

@@ -357,7 +357,7 @@ CB200_API int cb200_embedding_scaled(const void* table, const void* ids, void* o
  *   out[v, :]  = T(out[v, :] + scale * that sum), rows that no id names left alone       accumulate != 0
  * grad is [n_ids, hidden] with rows `grad_stride` elements apart (0 <= grad_stride; 0 is one row for all ids), out
  * [vocab, hidden] of `out_dtype`: `dtype` or F32.  With accumulate == 0 every row of `out` is written (zeros
- * where no id points).  Tokens whose id is `padding_id` contribute nothing (-1: there is none); ids outside
+ * where no id points).  Tokens whose id is `padding_id`, a row of the table, contribute nothing (-1: there is none); ids outside
  * the table contribute nothing and are reported.  `out` overlaps neither grad nor ids.
  * The tokens are brought into the order of their ids (stable, so the sums have a fixed order).
  * n_ids and vocab are below 2^31.

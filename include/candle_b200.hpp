@@ -341,7 +341,7 @@ inline int64_t embedding_backward_workspace(int64_t vocab, int64_t hidden, int64
 }
 
 /* out[v] = scale * sum of the rows of grad whose id is v, or with `accumulate` added to out; grad is ids.dims ++ [hidden], out
- * [vocab, hidden] of grad's type or F32; tokens of `padding_id` (-1: none) contribute nothing. */
+ * [vocab, hidden] of grad's type or F32; tokens of `padding_id`, a row (-1: none), contribute nothing. */
 inline void embedding_backward(const Tensor& grad, const Tensor& ids, Tensor& out, Workspace workspace, cb200_status* status,
                                cb200_stream_t stream, float scale = 1.0f, bool accumulate = false, int64_t padding_id = -1) {
   if (!is_float(grad.dtype)) throw Error(std::string("unsupported dtype ") + dtype_name(grad.dtype) + " for embedding-backward");

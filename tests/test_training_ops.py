@@ -187,6 +187,24 @@ def test_c_entry_points_refuse_on_the_host():
         assert lib.cb200_qk_norm_rope_backward(*args) < 0, i
 
 
+def test_a_padding_id_is_a_row_of_the_table():
+    import ctypes
+
+    import candle_b200 as cb
+    from candle_b200 import _cabi
+
+    grad, ids = torch.zeros(3, 8), torch.tensor([1, -1, 2])
+    for padding in (-100, -1, 10, 1 << 40):  # of ids outside the table every one is reported, so none can be padding
+        with pytest.raises(cb.CandleError, match="padding_id"):
+            cb.embedding_backward(grad, ids, 10, padding_id=padding)
+    with pytest.raises(cb.CandleError, match="no CPU fallback"):
+        cb.embedding_backward(grad, ids, 10, padding_id=9)
+    one, n = ctypes.c_void_p(16), ctypes.c_int64()
+    assert _cabi.lib.cb200_embedding_backward_workspace(10, 8, 100, ctypes.addressof(n)) == 0
+    for padding in (-2, 10):
+        assert _cabi.lib.cb200_embedding_backward(one, 8, one, one, 10, 8, 100, 1.0, padding, 0, 0, 0, 1, one, n.value, None, None) == -1
+
+
 def test_cpp_mirror_compiles_and_refuses(tmp_path):
     import os
     import shutil
