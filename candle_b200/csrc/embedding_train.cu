@@ -5,15 +5,16 @@
 // fixed order: no floating-point atomics, equal inputs give equal bits.  Then
 //   - chunk_sums_kernel adds up every aligned chunk of 32 sorted tokens that belongs to one id: text is skewed
 //     (the hottest id of 65536 tokens has thousands) and this is what spreads a long run over the GPU;
-//   - long_runs_kernel adds these and the ends that do not fill a chunk, for runs of 64 tokens and more;
-//   - row_stream_kernel adds the other runs.  Work is cut by tokens, not by rows, since a few rows of a text's table have
-//     most of its tokens: a warp takes the runs that begin at a few neighbouring sorted positions.
+//   - row_stream_kernel adds the runs.  A CTA per SM begins with the long ones (64 tokens and more: their chunk sums and the
+//     ends that do not fill a chunk), whose chains of dependent loads the other CTAs' traffic hides.  For the others
+//     work is cut by tokens, not by rows, since a few rows of a text's table have most of its tokens: a warp takes the
+//     runs that begin at a few neighbouring sorted positions.
 // The rows without tokens are filled with zeros by further blocks of the launches that leave the memory idle: the radix
 // sort's, or with few tokens the chunk sums' or the row sums'.
 //
-// Measured (B200): 65536 Zipf-distributed tokens, 128256 x 4096 bf16 (537 MB of gradients in, 1051 MB out): 311 us, 5.1 TB/s;
-// 4096 tokens added to a 32000 x 4096 f32 table (160 MB): 44 us; 46 tokens, 81761 x 2504 f32 (819 MB of zeros): 119 us.
-// Below some 8000 tokens the time is the latency of the four to five launches.
+// Measured (B200): 65536 Zipf-distributed tokens, 128256 x 4096 bf16 (537 MB of gradients in, 1051 MB out): 298 us, 5.3 TB/s
+// (the long runs in a launch of their own: 312); 4096 tokens added to a 32000 x 4096 f32 table (160 MB): 43 us; 46 tokens,
+// 81761 x 2504 f32 (819 MB of zeros): 119 us.  Below some 8000 tokens the time is the latency of the three to four launches.
 #include "launch.h"
 
 namespace cb200 {
@@ -205,6 +206,11 @@ __device__ __forceinline__ void fill_rows(const ZeroFill& z, unsigned block) {
 //   moves the keys: every CTA derives from all the counts where its keys of each digit go, and counts the next digit
 //   for the CTA that will read them.  A CTA takes a contiguous span of keys in tiles of 2048.
 // ---------------------------------------------------------------------------------------------
+struct Counters {
+  unsigned long long next_item;  // items of the row sums that warps took beyond their first
+  uint32_t n_long;               // long runs listed
+};
+
 constexpr int kSortItems = 4;
 constexpr int kSortThreads = 512;
 constexpr int kSortTile = kSortThreads * kSortItems;
@@ -223,7 +229,7 @@ struct SortArgs {
   uint32_t* values_out;
   uint32_t* counts;          // [ctas][bins] of this digit
   uint32_t* next_counts;     // of the next one; NULL at the last
-  uint32_t* n_long;          // number of long runs: cleared by the sort's first launch
+  Counters* counters;        // cleared by the sort's first launch
   ZeroFill zero;
   unsigned sort_blocks;      // the first blocks; the zero-filling ones follow
   int64_t n;
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs
   if (threadIdx.x < bins) hist[threadIdx.x] = 0;
   marked[threadIdx.x] = 0xFFFFFFFFu;
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_long = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.counters = Counters{};
   const int64_t begin = blockIdx.x * a.span;
   const int64_t end = begin + a.span < a.n ? begin + a.span : a.n;
   for (int64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(kRankThreads) sort_small_kernel(const SortArgs
   __shared__ uint32_t part[kRankWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = static_cast<int>(a.n);
   const int first = static_cast<int>(blockIdx.x) * 32;  // this block's tokens
-  if (first == 0 && threadIdx.x == 0) *a.n_long = 0;
+  if (first == 0 && threadIdx.x == 0) *a.counters = Counters{};
   const int padded = (n + 31) / 32 * 32;
 #pragma unroll 8
   for (int i = threadIdx.x; i < padded; i += kRankThreads) words[i] = i < n ? key_of_id(a.tokens, i, false) : 0xFFFFFFFFu;
@@ -422,7 +428,7 @@ struct SumArgs {
   const uint32_t* keys;    // sorted
   const uint32_t* tokens;  // their positions
   float* chunk_sums;       // [n / kChunk][hidden]
-  uint32_t* n_long;        // number of long runs
+  Counters* counters;
   uint2* long_runs;        // {one past its last sorted index, id} of each, in no particular order
   uint32_t* begins;        // [vocab] where the long runs begin; nothing for other ids
   void* out;
@@ -432,6 +438,8 @@ struct SumArgs {
   int units;               // VEC-element units per row
   int tiles;               // tiles of 32 units per row
   int group;               // sorted positions per warp and visit
+  unsigned long_blocks;    // the launch's first blocks, which begin with the long runs
+  int share;               // how the items of the row sums are shared out
   ZeroFill zero;
 };
 constexpr int kChunkBatch = 8;
@@ -473,7 +481,7 @@ __global__ void __launch_bounds__(256) chunk_sums_kernel(const __grid_constant__
     if (key >= a.vocab || a.keys[i + kLongRun - 1] != key) continue;
     if (i == 0 || a.keys[i - 1] != key) a.begins[key] = static_cast<uint32_t>(i);
     const int64_t behind = i + kLongRun;  // of the 64 positions from i on
-    if (behind == a.n || a.keys[behind] != key) a.long_runs[atomicAdd(a.n_long, 1u)] = make_uint2(static_cast<uint32_t>(behind), key);
+    if (behind == a.n || a.keys[behind] != key) a.long_runs[atomicAdd(&a.counters->n_long, 1u)] = make_uint2(static_cast<uint32_t>(behind), key);
   }
   const int tiles = (a.units + 32 * C - 1) / (32 * C);
   const int64_t n_items = a.n / kChunk * tiles;
@@ -599,14 +607,16 @@ __device__ __forceinline__ void finish_run(const SumArgs& a, uint32_t key, int u
   write_unit<DTO, VEC, ACC>(a, key, u, acc, old);
 }
 
-// The long runs.  Bound by the latency of dependent loads (list, positions, rows): 87 runs of 4096 columns take 22 us.
+// The long runs, by the launch's first long_blocks CTAs.  Bound by the latency of dependent loads (list, positions, rows).
 // With chunk sums and many of them: eight (run, tile) items per CTA at a time, a warp for each run of fewer
-// than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.
+// than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.  (Eight
+// at a time for 1400 items on 148 CTAs: the hottest runs' tiles end up in one CTA, 341 us for the call instead of 298.)
 constexpr int kWarpRun = 512;
+template <int VEC>
+constexpr size_t kLongShared = size_t(8) * 32 * VEC * 4 + size_t(8) * kPieces * PieceRing<VEC>::kWords * 32 * 16;
 template <int DT, int DTO, int VEC, bool ACC>
-__global__ void __launch_bounds__(256, 3) long_runs_kernel(const __grid_constant__ SumArgs a) {
-  follow_previous();
-  extern __shared__ __align__(16) unsigned char shared[];
+__device__ __forceinline__ void long_runs(const SumArgs& a, unsigned char* shared) {
+  const int blocks = a.long_blocks, block = static_cast<int>(blockIdx.x);
   float(*part)[32 * VEC] = reinterpret_cast<float(*)[32 * VEC]>(shared);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* ring = reinterpret_cast<uint4*>(shared + 8 * 32 * VEC * 4) + warp * (kPieces * PieceRing<VEC>::kWords * 32) + lane;
@@ -626,9 +636,9 @@ __global__ void __launch_bounds__(256, 3) long_runs_kernel(const __grid_constant
     __syncthreads();
   };
   if (a.chunk_sums != nullptr) {
-    const int64_t n_items = static_cast<int64_t>(*a.n_long) * a.tiles;
-    const int together = n_items > 4 * static_cast<int64_t>(gridDim.x) ? 8 : 1;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * together; base < n_items; base += static_cast<int64_t>(gridDim.x) * together) {
+    const int64_t n_items = static_cast<int64_t>(a.counters->n_long) * a.tiles;
+    const int together = n_items > 12 * static_cast<int64_t>(blocks) ? 8 : 1;
+    for (int64_t base = static_cast<int64_t>(block) * together; base < n_items; base += static_cast<int64_t>(blocks) * together) {
       if (together > 1) {
         const int64_t mine = base + warp;
         bool big = false;
@@ -654,17 +664,20 @@ __global__ void __launch_bounds__(256, 3) long_runs_kernel(const __grid_constant
     return;
   }
   // no list: a long run holds a multiple of kLongRun, and the block of the first one takes it
-  const int64_t at = static_cast<int64_t>(blockIdx.x / a.tiles) * kLongRun;
-  const uint32_t key = a.keys[at];
-  if (key >= a.vocab || (at > 0 && a.keys[at - kLongRun] == key)) return;
-  int64_t begin = at;  // back to where the run begins, at most 63 positions
-  for (int k = 0; k < 2; ++k) {
-    const int64_t p = at - 1 - 32 * k - lane;
-    const unsigned other = ~__ballot_sync(0xFFFFFFFFu, p >= 0 && a.keys[p >= 0 ? p : 0] == key);
-    begin = at - 32 * k - (other ? __ffs(other) - 1 : 32);
-    if (other) break;
+  const int64_t n_items = (a.n + kLongRun - 1) / kLongRun * a.tiles;
+  for (int64_t item = block; item < n_items; item += blocks) {
+    const int64_t at = item / a.tiles * kLongRun;
+    const uint32_t key = a.keys[at];
+    if (key >= a.vocab || (at > 0 && a.keys[at - kLongRun] == key)) continue;
+    int64_t begin = at;  // back to where the run begins, at most 63 positions
+    for (int k = 0; k < 2; ++k) {
+      const int64_t p = at - 1 - 32 * k - lane;
+      const unsigned other = ~__ballot_sync(0xFFFFFFFFu, p >= 0 && a.keys[p >= 0 ? p : 0] == key);
+      begin = at - 32 * k - (other ? __ffs(other) - 1 : 32);
+      if (other) break;
+    }
+    if (begin + kLongRun <= a.n && a.keys[begin + kLongRun - 1] == key) by_cta(begin, run_end(a, begin), key, static_cast<int>(item % a.tiles));
   }
-  if (begin + kLongRun <= a.n && a.keys[begin + kLongRun - 1] == key) by_cta(begin, run_end(a, begin), key, static_cast<int>(blockIdx.x % a.tiles));
 }
 
 // The runs that begin in a group of sorted positions show in the keys of the positions themselves and of the 63 behind
@@ -722,8 +735,10 @@ struct Stretch {
 // The blocks of row_stream_kernel and its like: the ones that sum and the zero-filling ones take turns, as far as there are
 // both, so that they share the SMs.  Whether this is a zero-filling one; `block` becomes its index among its kind.
 __device__ __forceinline__ bool take_turns(const SumArgs& a, unsigned& block) {
-  const unsigned sums = gridDim.x - a.zero.blocks, both = sums < a.zero.blocks ? sums : a.zero.blocks;
+  if (block < a.long_blocks) return false;
+  const unsigned sums = gridDim.x - a.long_blocks - a.zero.blocks, both = sums < a.zero.blocks ? sums : a.zero.blocks;
   bool fill;
+  block -= a.long_blocks;
   if (block < 2 * both) {
     fill = block & 1u;
     block >>= 1;
@@ -733,6 +748,31 @@ __device__ __forceinline__ bool take_turns(const SumArgs& a, unsigned& block) {
   }
   return fill;
 }
+
+// The items of a warp of the row sums.  The first is its own.  With `share` each then takes the next that nobody has,
+// since runs differ in length and the blocks that began with the long runs come late (these take their first one so as
+// well); without, it takes every so-manieth and those blocks none: few tokens make small items, and thousands of warps
+// that count in one place at the same time wait for one another.
+struct Items {
+  unsigned long long claimed = 0;  // lane 0: the item after the current one, asked for an item ahead
+  int64_t fixed, n_items;          // items that are somebody's own, all items
+  __device__ __forceinline__ void claim(const SumArgs& a) {
+    if ((threadIdx.x & 31) == 0 && fixed < n_items) claimed = atomicAdd(&a.counters->next_item, 1ull);
+  }
+  __device__ __forceinline__ int64_t next(const SumArgs& a, int64_t item) {
+    if (!a.share) return item + fixed;
+    item = fixed + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, claimed, 0));
+    claim(a);
+    return item;
+  }
+  __device__ __forceinline__ int64_t first(const SumArgs& a, int64_t n, unsigned block) {
+    n_items = n;
+    fixed = static_cast<int64_t>(gridDim.x - a.long_blocks - a.zero.blocks) * 8;
+    if (a.share) claim(a);
+    if (blockIdx.x < a.long_blocks) return a.share ? next(a, 0) : n;
+    return static_cast<int64_t>(block) * 8 + (threadIdx.x >> 5);
+  }
+};
 
 template <bool ACC, int V>
 struct Ring {
@@ -750,18 +790,22 @@ __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __gr
   extern __shared__ __align__(16) unsigned char shared[];
   unsigned block = blockIdx.x;
   if (take_turns(a, block)) return fill_rows(a.zero, block);
+  if (blockIdx.x < a.long_blocks) {
+    long_runs<DT, DTO, VEC, ACC>(a, shared);
+    __syncthreads();  // the shared memory changes its use
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* ring = reinterpret_cast<uint4*>(shared) + warp * (Ring<ACC, V>::kDepth * kSlot * 32) + lane;  // [slot][word][lane]
   const int row_tiles = (a.units + 32 * V - 1) / (32 * V);
   const int64_t n_items = (a.n + a.group - 1) / a.group * row_tiles;
-  const int64_t stride = static_cast<int64_t>(gridDim.x - a.zero.blocks) * 8;
 
-  int64_t item = static_cast<int64_t>(block) * 8 + warp;  // the next one to be opened; its window is on the way
+  Items items;
+  int64_t item = items.first(a, n_items, block);  // the next one to be opened; its window is on the way
   Window ahead, now;
   Stretch s;
   s.from = s.to = 0;
   int p = 0, tile = 0;
-  ahead.load(a, item / row_tiles * a.group);
+  ahead.load(a, item < n_items ? item / row_tiles * a.group : a.n);
   uint32_t slot_row = 0, slot_end = 0, slot_tile = 0;  // lane k: of the token in slot k
   unsigned issued = 0, done = 0;
 
@@ -769,7 +813,7 @@ __global__ void __launch_bounds__(256, ACC ? 2 : 3) row_stream_kernel(const __gr
     while (p == s.to && item < n_items) {
       now = ahead;
       tile = static_cast<int>(item % row_tiles);
-      item += stride;
+      item = items.next(a, item);
       ahead.load(a, item < n_items ? item / row_tiles * a.group : a.n);
       s.find(a, now);
       p = s.from;
@@ -846,13 +890,15 @@ constexpr int kAny = 4;
 template <int DT, int DTO, bool ACC>
 __global__ void __launch_bounds__(256, 3) row_sums_any_kernel(const __grid_constant__ SumArgs a) {
   follow_previous();
+  extern __shared__ __align__(16) unsigned char shared[];
   unsigned block = blockIdx.x;
   if (take_turns(a, block)) return fill_rows(a.zero, block);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x < a.long_blocks) long_runs<DT, DTO, 1, ACC>(a, shared);
+  const int lane = threadIdx.x & 31;
   const int row_tiles = (a.units + 32 * kAny - 1) / (32 * kAny);
   const int64_t n_items = (a.n + a.group - 1) / a.group * row_tiles;
-  const int64_t n_warps = static_cast<int64_t>(gridDim.x - a.zero.blocks) * 8;
-  for (int64_t item = static_cast<int64_t>(block) * 8 + warp; item < n_items; item += n_warps) {
+  Items items;
+  for (int64_t item = items.first(a, n_items, block); item < n_items; item = items.next(a, item)) {
     const int64_t group = item / row_tiles;
     const int u0 = static_cast<int>(item - group * row_tiles) * (32 * kAny) + lane;
     Window w;
@@ -893,7 +939,7 @@ int64_t round16(int64_t bytes) { return (bytes + 15) & ~int64_t(15); }
 
 struct Workspace {
   uint32_t *keys[2], *values[2], *counts[2];
-  uint32_t* n_long;
+  Counters* counters;
   uint2* long_runs;
   uint32_t* begins;
   unsigned char* present;
@@ -914,7 +960,7 @@ Workspace lay_out(void* base, int64_t vocab, int hidden, int64_t n) {
     w.values[i] = reinterpret_cast<uint32_t*>(take(n * 4));
     w.counts[i] = reinterpret_cast<uint32_t*>(take(int64_t(kSortMaxCtas) * kSortMaxBins * 4));
   }
-  w.n_long = reinterpret_cast<uint32_t*>(take(4));
+  w.counters = reinterpret_cast<Counters*>(take(sizeof(Counters)));
   w.long_runs = reinterpret_cast<uint2*>(take(n / kLongRun * 8));
   w.begins = reinterpret_cast<uint32_t*>(take(vocab * 4));
   w.present = take(vocab);
@@ -943,7 +989,7 @@ cudaError_t sort_tokens(const TableGradArgs& a, const Workspace& w, int* where, 
   SortArgs s{};
   s.tokens = Ids{a.ids, a.n_ids, a.vocab, a.padding_id, a.id_dtype, a.status};
   s.n = a.n_ids;
-  s.n_long = w.n_long;
+  s.counters = w.counters;
   if (rest.end > 0) {
     const cudaError_t e = cudaMemsetAsync(w.present, 0, static_cast<size_t>(a.vocab), stream);
     if (e != cudaSuccess) return e;
@@ -994,7 +1040,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
   s.grad_stride = a.grad_stride;
   s.keys = w.keys[where];
   s.tokens = w.values[where];
-  s.n_long = w.n_long;
+  s.counters = w.counters;
   s.long_runs = w.long_runs;
   s.begins = w.begins;
   s.out = a.out;
@@ -1019,17 +1065,9 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     if (e != cudaSuccess) return e;
   }
   s.zero = share_of(rest, rest.end - rest.begin);
-  if (a.n_ids >= kLongRun) {
-    // with a list three CTAs per SM share it out
-    constexpr size_t smem = size_t(8) * 32 * VEC * 4 + size_t(8) * kPieces * PieceRing<VEC>::kWords * 32 * 16;
-    cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(long_runs_kernel<DT, DTO, VEC, ACC>), 256, smem, -1, nullptr);
-    if (e != cudaSuccess) return e;
-    const int64_t blocks = chunks ? a.n_ids / kLongRun * s.tiles : (a.n_ids + kLongRun - 1) / kLongRun * s.tiles;
-    e = launch_dependent(few, long_runs_kernel<DT, DTO, VEC, ACC>, static_cast<unsigned>(chunks && blocks > 3 * sms ? 3 * sms : blocks), 256, smem, stream, s);
-    if (e != cudaSuccess) return e;
-  }
   const auto finish = [&](auto kern, int vectors, size_t smem) {
     int per_sm = 4;
+    if (smem < kLongShared<VEC>) smem = kLongShared<VEC>;
     const cudaError_t e = kernel_launch_config(reinterpret_cast<const void*>(kern), 256, smem, -1, &per_sm);
     if (e != cudaSuccess) return e;
     // a few items per warp that is resident at once, so that the uneven runs even out; few tokens: few positions per item
@@ -1037,8 +1075,13 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     s.group = kMaxGroup;
     while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * tiles < sms * per_sm * 8 * 4) s.group /= 2;
     const int64_t items = (a.n_ids + s.group - 1) / s.group * tiles;
-    const int64_t token_blocks = (items + 7) / 8 < sms * per_sm ? (items + 7) / 8 : sms * per_sm;
-    return launch_dependent(few, kern, static_cast<unsigned>(token_blocks) + s.zero.blocks, 256, smem, stream, s);
+    // a CTA per SM begins with the long runs, if there are any (two: 305 instead of 298 us for 65536 skewed tokens)
+    const int64_t long_items = a.n_ids < kLongRun ? 0 : (chunks ? a.n_ids / kLongRun : (a.n_ids + kLongRun - 1) / kLongRun) * s.tiles;
+    s.long_blocks = static_cast<unsigned>(long_items < sms ? long_items : sms);
+    s.share = few ? 0 : 1;
+    const int64_t room = sms * (per_sm > 1 ? per_sm : 2) - (s.share ? s.long_blocks : 0);
+    const int64_t blocks = (items + 7) / 8 < room ? (items + 7) / 8 : room;
+    return launch_dependent(few, kern, s.long_blocks + static_cast<unsigned>(blocks) + s.zero.blocks, 256, smem, stream, s);
   };
   if constexpr (VEC > 1) {
     // Several vectors per lane share what a token costs in instructions (1 -> 4 vectors: 120 -> 95 us for the sums of
