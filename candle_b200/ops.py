@@ -450,10 +450,13 @@ if _raw_stream is not None:
     def _stream_of(device: torch.device) -> int:  # noqa: F811
         return _raw_stream(device.index)
 
+# and the current device's number: every call has a tensor of the device, so there is nothing to initialise
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
 
 def _launch(device: torch.device, name: str, *args) -> None:
     """The entry point `name` on `device`'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         _cabi.call(name, *args, _stream_of(device))
     else:
         with torch.cuda.device(device):
@@ -475,8 +478,12 @@ def _workspace(device: torch.device, name: str, *args) -> tuple[torch.Tensor, in
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
     """First and one-past-last byte address of a tensor with non-negative strides."""
-    if t.numel() == 0:
+    n = t.numel()
+    if n == 0:
         return 0, 0
+    if t.is_contiguous():
+        at = t.data_ptr()
+        return at, at + n * t.element_size()
     last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
@@ -524,7 +531,7 @@ def embedding_scaled(table: torch.Tensor, ids: torch.Tensor, scale: float, *, ou
         raise CandleError("index-select requires contiguous tensors")
     if table.dtype not in _DTYPES:
         raise CandleError(f"unsupported dtype {table.dtype} for embedding")
-    flat = _ids_checks(ids.reshape(-1))
+    flat = _ids_checks(ids if ids.dim() == 1 else ids.reshape(-1))
     _same_device(table, flat, out)
     vocab, hidden = table.shape
     final = [*ids.shape, hidden]
@@ -555,16 +562,18 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     of the table, contribute nothing."""
     if grad.dtype not in _DTYPES:
         raise CandleError(f"unsupported dtype {grad.dtype} for embedding-backward")
-    if grad.dim() == 0 or list(grad.shape[:-1]) != list(ids.shape):
+    shape = grad.shape
+    if len(shape) == 0 or shape[:-1] != ids.shape:
         raise CandleError(f"shape mismatch in embedding-backward {_dims(grad)} {_dims(ids)}")
-    hidden = grad.shape[-1]
-    flat = _ids_checks(ids.reshape(-1))
+    hidden = shape[-1]
+    flat = _ids_checks(ids if ids.dim() == 1 else ids.reshape(-1))
     n = flat.shape[0]
     try:
-        rows = grad.view(n, hidden)
+        rows = grad if len(shape) == 2 else grad.view(n, hidden)
     except RuntimeError:
         raise CandleError("the rows of grad must have one stride in embedding-backward") from None
-    if hidden > 1 and rows.stride(1) != 1:
+    row_stride, column_stride = rows.stride()
+    if hidden > 1 and column_stride != 1:
         raise CandleError("the last dimension of grad has to be contiguous in embedding-backward")
     vocab = int(vocab)
     if vocab < 0:
@@ -581,12 +590,12 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
             raise CandleError("embedding-backward accumulates into `out`, which is missing")
         out = torch.empty(vocab, hidden, dtype=out_dtype, device=grad.device)
     else:
-        if list(out.shape) != [vocab, hidden] or out.dtype != out_dtype or not out.is_contiguous():
+        if out.shape != (vocab, hidden) or out.dtype != out_dtype or not out.is_contiguous():
             raise CandleError(f"out must be a contiguous {out_dtype} tensor of shape {[vocab, hidden]}, got {out.dtype} {_dims(out)}")
         _check_apart("embedding-backward", out, rows, flat, same=False)
     ws, ws_bytes = _workspace(grad.device, "cb200_embedding_backward_workspace", vocab, hidden, n)
     st = status if status is not None else (new_status(grad.device) if check else None)
-    _launch(grad.device, "cb200_embedding_backward", _ptr(rows), rows.stride(0) if n > 1 else hidden, _ptr(flat), _ptr(out),
+    _launch(grad.device, "cb200_embedding_backward", _ptr(rows), row_stride if n > 1 else hidden, _ptr(flat), _ptr(out),
             vocab, hidden, n, float(scale), -1 if padding_id is None else int(padding_id), 1 if accumulate else 0,
             _DTYPES[grad.dtype], _DTYPES[out_dtype], _ID_DTYPES[flat.dtype], _ptr(ws), ws_bytes, _ptr(st))
     if check:
@@ -594,12 +603,8 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     return out
 
 
-def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor, eps: float, *,
-                      grad_sum: torch.Tensor | None = None, out: torch.Tensor | None = None):
-    """Gradient of ``rms_norm(xs, alpha, eps)``: ``(dxs, dalpha)`` for the gradient ``grad`` of its result, ``dalpha`` in
-    f32.  After ``rms_norm(x, alpha, eps, residual=r, return_sum=True)`` pass the returned sum as ``xs`` and the gradient
-    that reaches that sum on the residual stream as ``grad_sum``, which is added: ``dxs`` is then the gradient of both
-    ``x`` and ``r``.  ``out`` may be ``grad``, ``xs`` or ``grad_sum``."""
+def _rms_backward_refuse(grad, xs, alpha, grad_sum) -> None:
+    """Raises what is wrong with the arguments of the RMS norm's gradient."""
     if xs.dim() == 0:
         raise CandleError("unexpected rank, expected: at least 1, got: 0")
     if alpha.dim() != 1:
@@ -615,6 +620,23 @@ def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor,
             raise CandleError("the gradient has to be contiguous")
     _norm_checks("rms-norm", xs, [("alpha", alpha)], None)
     _same_device(xs, grad, grad_sum)
+
+
+def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor, eps: float, *,
+                      grad_sum: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """Gradient of ``rms_norm(xs, alpha, eps)``: ``(dxs, dalpha)`` for the gradient ``grad`` of its result, ``dalpha`` in
+    f32.  After ``rms_norm(x, alpha, eps, residual=r, return_sum=True)`` pass the returned sum as ``xs`` and the gradient
+    that reaches that sum on the residual stream as ``grad_sum``, which is added: ``dxs`` is then the gradient of both
+    ``x`` and ``r``.  ``out`` may be ``grad``, ``xs`` or ``grad_sum``."""
+    t, shape, dev = xs.dtype, xs.shape, xs.get_device()
+    if not (
+        t in _DTYPES and len(shape) > 0 and alpha.shape == shape[-1:] and alpha.dtype == t and grad.shape == shape and grad.dtype == t
+        and xs.is_contiguous() and alpha.is_contiguous() and grad.is_contiguous()
+        and dev >= 0 and alpha.get_device() == dev and grad.get_device() == dev
+        and (grad_sum is None or grad_sum.shape == shape and grad_sum.dtype == t and grad_sum.is_contiguous()
+             and grad_sum.get_device() == dev)
+    ):
+        _rms_backward_refuse(grad, xs, alpha, grad_sum)
     dx = _out_check(out, xs)
     if out is not None:
         _check_apart("rms-norm-backward", out, grad, xs, grad_sum)
@@ -630,6 +652,10 @@ def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor,
 
 _HEADS = struct.Struct("=qqqqii")  # cb200_heads
 _QK_ARGS = struct.Struct("=qqqqqqqqiifiiiii")  # cb200_qk_args
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _heads(t: torch.Tensor, rank: int, heads: int) -> bytes:
@@ -727,7 +753,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     args, rank, q_heads, k_heads, _, device = _qk_args("qk-norm-rope", q, k, q_weight, k_weight, eps, cos, sin, positions,
                                                        interleaved, more)
     if out is None:
-        q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+        q_out, k_out = _fresh(q), _fresh(k)
     else:
         q_out, k_out = out
         _check_apart("qk-norm-rope", q_out, q)
@@ -758,7 +784,7 @@ def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.T
     args, rank, q_heads, k_heads, dim, device = _qk_args(op, q, k, q_weight, k_weight, eps, cos, sin, positions, interleaved,
                                                          more)
     if out is None:
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        dq, dk = _fresh(q), _fresh(k)
     else:
         dq, dk = out
         _check_apart(op, dq, q, grad_q)
