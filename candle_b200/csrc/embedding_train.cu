@@ -609,8 +609,9 @@ __device__ __forceinline__ void finish_run(const SumArgs& a, uint32_t key, int u
 
 // The long runs, by the launch's first long_blocks CTAs.  Bound by the latency of dependent loads (list, positions, rows).
 // With chunk sums and many of them: eight (run, tile) items per CTA at a time, a warp for each run of fewer
-// than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.  (Eight
-// at a time for 1400 items on 148 CTAs: the hottest runs' tiles end up in one CTA, 341 us for the call instead of 298.)
+// than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.  The eight
+// lie far apart in the list, so that the tiles of a hot run go to different CTAs (65536 tokens over 1000 rows of
+// 8192: 343 us with neighbours, 284 so).
 constexpr int kWarpRun = 512;
 template <int VEC>
 constexpr size_t kLongShared = size_t(8) * 32 * VEC * 4 + size_t(8) * kPieces * PieceRing<VEC>::kWords * 32 * 16;
@@ -637,10 +638,11 @@ __device__ __forceinline__ void long_runs(const SumArgs& a, unsigned char* share
   };
   if (a.chunk_sums != nullptr) {
     const int64_t n_items = static_cast<int64_t>(a.counters->n_long) * a.tiles;
-    const int together = n_items > 12 * static_cast<int64_t>(blocks) ? 8 : 1;
-    for (int64_t base = static_cast<int64_t>(block) * together; base < n_items; base += static_cast<int64_t>(blocks) * together) {
-      if (together > 1) {
-        const int64_t mine = base + warp;
+    const bool together = n_items > 12 * static_cast<int64_t>(blocks);
+    const int64_t batches = together ? (n_items + 7) / 8 : n_items;  // batch b: the items b, b + batches, ...
+    for (int64_t batch = block; batch < batches; batch += blocks) {
+      if (together) {
+        const int64_t mine = batch + warp * batches;
         bool big = false;
         if (mine < n_items) {
           const uint2 run = a.long_runs[mine / a.tiles];
@@ -655,10 +657,10 @@ __device__ __forceinline__ void long_runs(const SumArgs& a, unsigned char* share
         }
         if (!__syncthreads_or(big)) continue;
       }
-      for (int64_t item = base; item < base + together && item < n_items; ++item) {
+      for (int64_t item = batch; item < n_items; item += batches) {
         const uint2 run = a.long_runs[item / a.tiles];
         const int64_t begin = a.begins[run.y];
-        if (together == 1 || run.x - begin >= kWarpRun) by_cta(begin, run.x, run.y, static_cast<int>(item % a.tiles));
+        if (!together || run.x - begin >= kWarpRun) by_cta(begin, run.x, run.y, static_cast<int>(item % a.tiles));
       }
     }
     return;
