@@ -1086,16 +1086,11 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     return launch_dependent(few, kern, s.long_blocks + static_cast<unsigned>(blocks) + s.zero.blocks, 256, smem, stream, s);
   };
   if constexpr (VEC > 1) {
-    // Several vectors per lane share what a token costs in instructions (1 -> 4 vectors: 120 -> 95 us for the sums of
-    // 65536 skewed tokens of 4096 columns), one keeps more tokens of a run in flight and more warps busy (3001 tokens
-    // of 1000 columns: 32 -> 18 us).
+    // Two vectors per lane share what a token costs in instructions (65536 skewed tokens of 4096 columns: 341 us with one,
+    // 297 with two); one keeps more warps busy where there are not four such items for each.  Four make the items so
+    // large that the last ones are waited for: 115 us instead of 104 for 16384 tokens.
     constexpr size_t kSmem = size_t(8) * (ACC ? 8 : 16) * 32 * (16 + (ACC ? VEC * Elem<DTO>::kBytes : 0));
-    const auto enough = [&](int vectors, int per_warp) {
-      return s.units > 16 * vectors && a.n_ids * ((s.units + 32 * vectors - 1) / (32 * vectors)) >= sms * 24 * per_warp;
-    };
-    if constexpr (!ACC)
-      if (enough(4, 16)) return finish(row_stream_kernel<DT, DTO, ACC, 4>, 4, kSmem);
-    if (enough(2, 8)) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
+    if (s.units > 32 && a.n_ids * ((s.units + 63) / 64) >= sms * 24 * 4) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
     return finish(row_stream_kernel<DT, DTO, ACC, 1>, 1, kSmem);
   } else {
     return finish(row_sums_any_kernel<DT, DTO, ACC>, kAny, 0);
