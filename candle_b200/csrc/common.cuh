@@ -175,32 +175,6 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// The pairs of a 16-byte vector, widened, and back (each rounded once to T).
-template <int DT>
-__device__ __forceinline__ void vec_to_pairs(const uint4& q, F2 (&f)[Elem<DT>::kPerVec / 2]) {
-  if constexpr (DT == kDtF32) {
-    f[0] = pair(__uint_as_float(q.x), __uint_as_float(q.y));
-    f[1] = pair(__uint_as_float(q.z), __uint_as_float(q.w));
-  } else {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = unpack2<DT>(w[i]);
-      f[i] = pair(t.x, t.y);
-    }
-  }
-}
-template <int DT>
-__device__ __forceinline__ uint4 pairs_to_vec(const F2 (&f)[Elem<DT>::kPerVec / 2]) {
-  float t[Elem<DT>::kPerVec];
-#pragma unroll
-  for (int i = 0; i < Elem<DT>::kPerVec / 2; ++i) {
-    const float2 u = unpair(f[i]);
-    t[2 * i] = u.x;
-    t[2 * i + 1] = u.y;
-  }
-  return floats_to_vec<DT>(t);
-}
 
 // What a vocabulary shard writes for a row it does not own: zero BITS.  The shards' partial rows are
 // combined by adding their bit patterns as unsigned integers (one non-zero contributor per element),
