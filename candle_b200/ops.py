@@ -494,14 +494,14 @@ def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
     if a.dtype != b.dtype:
         return False
     size = a.element_size()
-    for step in set(a.stride()) & set(b.stride()):
+    for step in set(a.stride()) & set(b.stride()) - {0}:  # a broadcast dimension sets nothing apart
         inner = []
         for t in (a, b):
             dims = [(n, st) for n, st in zip(t.shape, t.stride()) if n > 1]
             if any(st >= step and st % step for _, st in dims):
                 break
             inner.append(1 + sum((n - 1) * st for n, st in dims if st < step))
-        at, rest = divmod((b.data_ptr() - a.data_ptr()) % (step * size), size) if step else (0, 1)
+        at, rest = divmod((b.data_ptr() - a.data_ptr()) % (step * size), size)
         if len(inner) == 2 and rest == 0 and inner[0] <= at and at + inner[1] <= step:
             return True
     return False

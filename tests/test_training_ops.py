@@ -143,6 +143,20 @@ def test_overlapping_outputs_are_told_apart():
         _check_apart("x", flat[:51], flat[50:])
 
 
+def test_overlapping_views_with_broadcast_dimensions_are_refused():
+    from candle_b200 import CandleError
+    from candle_b200.ops import _check_apart
+
+    b = torch.zeros(12)
+    rows = torch.zeros(3, 8)
+    for x, y in ((b[:8].expand(4, 8), b[4:12].expand(4, 8)), (b[:8].expand(1, 8), b[4:12].expand(4, 8)),
+                 (b[:8].expand(2, 4, 8), b[7:].expand(2, 4, 5)), (rows[:2, None].expand(2, 4, 8), rows[1:, None].expand(2, 4, 8))):
+        with pytest.raises(CandleError, match="overlaps"):
+            _check_apart("x", x, y)
+    # columns of the same rows, each read for all heads
+    _check_apart("x", rows[:, None, :4].expand(3, 4, 4), rows[:, None, 4:].expand(3, 4, 4), same=False)
+
+
 def test_c_entry_points_refuse_on_the_host():
     import ctypes
     import struct
