@@ -516,7 +516,8 @@ def _check_apart(op: str, out: torch.Tensor, *others: torch.Tensor | None, same:
         a, b = _span(t)
         if hi <= a or b <= lo:
             continue
-        if same and t.data_ptr() == out.data_ptr() and t.stride() == out.stride() and t.shape == out.shape and t.dtype == out.dtype:
+        if same and t.data_ptr() == out.data_ptr() and t.shape == out.shape and t.dtype == out.dtype and all(
+                x == y for n, x, y in zip(t.shape, t.stride(), out.stride()) if n > 1):
             continue
         if not _interleaved(out, t):
             raise CandleError(f"the output of {op} overlaps another tensor of the call")

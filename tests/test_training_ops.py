@@ -157,6 +157,24 @@ def test_overlapping_views_with_broadcast_dimensions_are_refused():
     _check_apart("x", rows[:, None, :4].expand(3, 4, 4), rows[:, None, 4:].expand(3, 4, 4), same=False)
 
 
+def test_the_same_view_whatever_the_strides_of_its_single_dimensions():
+    from candle_b200 import CandleError
+    from candle_b200.ops import _check_apart
+
+    one = torch.zeros(6, 4, 16)  # a decoding step's heads: one token each, in two orders of the same memory
+    q, seen = one.unsqueeze(1), one.unsqueeze(2).transpose(1, 2)
+    assert q.shape == seen.shape and q.stride() != seen.stride()
+    _check_apart("x", q, seen)
+    _check_apart("x", seen[:1], q[:1])
+    row = torch.zeros(5, 64)
+    _check_apart("x", row[2:3], row[2:3].as_strided((1, 64), (7, 1), row[2:3].storage_offset()))
+    for other in (q[:, :, :3], q[1:], seen.transpose(1, 2), q.view(torch.int32)):
+        with pytest.raises(CandleError, match="overlaps"):
+            _check_apart("x", q, other)
+    with pytest.raises(CandleError, match="overlaps"):
+        _check_apart("x", q, seen, same=False)
+
+
 def test_c_entry_points_refuse_on_the_host():
     import ctypes
     import struct
