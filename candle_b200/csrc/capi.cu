@@ -141,18 +141,26 @@ int check_workspace(const char* name, const void* workspace, int64_t given, int6
   return CB200_OK;
 }
 
+// The kernels of the training operators count the columns of a row, and the heads of a token, in 32 bits: bytes of f32 columns
+// and rounding up to a tile included, that holds below 2^29.
+int check_counts(const char* name, int64_t count, const char* what) {
+  if (count >= (int64_t(1) << 29))
+    return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: %lld %s, they must be fewer than 2^29", name, (long long)count, what);
+  return CB200_OK;
+}
+
 int check_table_grad_shape(const char* name, int64_t vocab, int32_t hidden, int64_t n_ids) {
   if (vocab < 0 || hidden < 0 || n_ids < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape", name);
   if (vocab >= (int64_t(1) << 31) || n_ids >= (int64_t(1) << 31))
     return fail(CB200_E_UNSUPPORTED_SHAPE, "%s: the rows of the table and the ids must be fewer than 2^31", name);
-  return CB200_OK;
+  return check_counts(name, hidden, "columns");
 }
 
 int check_rms_backward_shape(const char* name, int64_t rows, int32_t cols) {
   if (rows < 0 || cols < 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: negative shape [%lld, %d]", name, (long long)rows, cols);
   if (cols == 0) return fail(CB200_E_INVALID_ARGUMENT, "%s: rows of zero columns cannot be normalised", name);
   if (rows > (int64_t(1) << 40)) return fail(CB200_E_INVALID_ARGUMENT, "%s: too many rows", name);
-  return CB200_OK;
+  return check_counts(name, cols, "columns");
 }
 
 int check_qk(const char* name, const cb200_qk_args* a) {
@@ -173,7 +181,12 @@ int check_qk(const char* name, const cb200_qk_args* a) {
                 (long long)a->max_positions);
   if (a->q_weight == nullptr || a->k_weight == nullptr || (a->max_positions > 0 && (a->cos == nullptr || a->sin == nullptr)))
     return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
-  return CB200_OK;
+  return check_counts(name, a->dim, "columns");
+}
+
+// The heads of a token, queries and keys together.
+int check_head_count(const char* name, const cb200_heads& q, const cb200_heads& k) {
+  return check_counts(name, int64_t(q.heads) + k.heads, "heads");
 }
 
 // `like`: the input whose heads `h` has to match; outputs may not map two elements to one address.
@@ -656,7 +669,8 @@ int cb200_embedding_scaled(const void* table, const void* ids, void* out, int64_
   const TraceRange trace("cb200_embedding_scaled");
   const char* name = "cb200_embedding_scaled";
   if (!valid_dtype(dtype)) return fail(CB200_E_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", name, dtype);
-  const int rc = check_lookup(name, table, ids, out, vocab, hidden, n_ids, id_dtype);
+  int rc = check_lookup(name, table, ids, out, vocab, hidden, n_ids, id_dtype);
+  if (rc == CB200_OK) rc = check_counts(name, hidden, "columns");
   if (rc != CB200_OK) return rc;
   cb200::ScaledLookupArgs a{};
   a.table = table;
@@ -766,12 +780,16 @@ int cb200_qk_norm_rope(const cb200_heads* q, const cb200_heads* k, const cb200_h
     if (rc == CB200_OK) rc = check_heads(name, out[i], in[i], args, true);
     if (rc != CB200_OK) return rc;
   }
+  rc = check_head_count(name, *q, *k);
+  if (rc != CB200_OK) return rc;
   return cuda_result(cb200::launch_qk_norm_rope(*q, *k, *q_out, *k_out, *args, status, stream), name);
 }
 
 int cb200_qk_norm_rope_backward_workspace(int32_t dim, int64_t* bytes) {
   const char* name = "cb200_qk_norm_rope_backward_workspace";
   if (dim < 0 || bytes == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: bad argument", name);
+  const int rc = check_counts(name, dim, "columns");
+  if (rc != CB200_OK) return rc;
   *bytes = cb200::qk_backward_workspace(dim);
   return CB200_OK;
 }
@@ -794,6 +812,8 @@ int cb200_qk_norm_rope_backward(const cb200_heads* grad_q, const cb200_heads* gr
     if (rc != CB200_OK) return rc;
   }
   if (dq_weight == nullptr || dk_weight == nullptr) return fail(CB200_E_INVALID_ARGUMENT, "%s: null tensor pointer", name);
+  rc = check_head_count(name, *q, *k);
+  if (rc != CB200_OK) return rc;
   rc = check_workspace(name, workspace, workspace_bytes, cb200::qk_backward_workspace(args->dim));
   if (rc != CB200_OK) return rc;
   return cuda_result(cb200::launch_qk_norm_rope_backward(*grad_q, *grad_k, *q, *k, *dq, *dk, static_cast<float*>(dq_weight),

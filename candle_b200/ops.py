@@ -440,6 +440,14 @@ def qembedding_route_rows(qtensor, ids: torch.Tensor, dst_ptrs, row_bounds, *, v
 # order, so equal inputs give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
 
 
+_COUNT_LIMIT = 1 << 29  # columns of a row, heads of a token: the kernels count them in 32 bits
+
+
+def _check_columns(op: str, columns: int) -> None:
+    if columns >= _COUNT_LIMIT:
+        raise CandleError(f"rows of {columns} columns in {op}, they must be fewer than 2^29")
+
+
 def _stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -533,8 +541,9 @@ def embedding_scaled(table: torch.Tensor, ids: torch.Tensor, scale: float, *, ou
     if table.dtype not in _DTYPES:
         raise CandleError(f"unsupported dtype {table.dtype} for embedding")
     flat = _ids_checks(ids if ids.dim() == 1 else ids.reshape(-1))
-    _same_device(table, flat, out)
     vocab, hidden = table.shape
+    _check_columns("embedding", hidden)
+    _same_device(table, flat, out)
     final = [*ids.shape, hidden]
     if out is None:
         out = torch.empty(final, dtype=table.dtype, device=table.device)
@@ -567,6 +576,7 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     if len(shape) == 0 or shape[:-1] != ids.shape:
         raise CandleError(f"shape mismatch in embedding-backward {_dims(grad)} {_dims(ids)}")
     hidden = shape[-1]
+    _check_columns("embedding-backward", hidden)
     flat = _ids_checks(ids if ids.dim() == 1 else ids.reshape(-1))
     n = flat.shape[0]
     try:
@@ -612,6 +622,7 @@ def _rms_backward_refuse(grad, xs, alpha, grad_sum) -> None:
         raise CandleError(f"unexpected rank, expected: 1, got: {alpha.dim()} ({_dims(alpha)})")
     if xs.shape[-1] != alpha.shape[0]:
         raise CandleError(f"shape mismatch in rms-norm {_dims(xs)} {_dims(alpha)}")
+    _check_columns("rms-norm-backward", alpha.shape[0])
     for g in (grad, grad_sum):
         if g is None:
             continue
@@ -631,7 +642,7 @@ def rms_norm_backward(grad: torch.Tensor, xs: torch.Tensor, alpha: torch.Tensor,
     ``x`` and ``r``.  ``out`` may be ``grad``, ``xs`` or ``grad_sum``."""
     t, shape, dev = xs.dtype, xs.shape, xs.get_device()
     if not (
-        t in _DTYPES and len(shape) > 0 and alpha.shape == shape[-1:] and alpha.dtype == t and grad.shape == shape and grad.dtype == t
+        t in _DTYPES and len(shape) > 0 and alpha.shape == shape[-1:] and shape[-1] < _COUNT_LIMIT and alpha.dtype == t and grad.shape == shape and grad.dtype == t
         and xs.is_contiguous() and alpha.is_contiguous() and grad.is_contiguous()
         and dev >= 0 and alpha.get_device() == dev and grad.get_device() == dev
         and (grad_sum is None or grad_sum.shape == shape and grad_sum.dtype == t and grad_sum.is_contiguous()
@@ -675,6 +686,9 @@ def _qk_refuse(op: str, q, k, q_weight, k_weight, cos, sin, positions, more) -> 
     d = q.shape[-1]
     if k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]:
         raise CandleError(f"shape mismatch in {op} {_dims(q)} {_dims(k)}")
+    _check_columns(op, d)
+    if q.shape[-2] + k.shape[-2] >= _COUNT_LIMIT:
+        raise CandleError(f"{q.shape[-2]} + {k.shape[-2]} heads in {op}, they must be fewer than 2^29")
     if q.dtype not in _DTYPES or any(t.dtype != q.dtype for t in (k, q_weight, k_weight)):
         raise CandleError(f"unsupported dtype for {op} {q.dtype} {k.dtype} {q_weight.dtype} {k_weight.dtype}")
     for w in (q_weight, k_weight):
@@ -717,7 +731,8 @@ def _qk_args(op: str, q, k, q_weight, k_weight, eps, cos, sin, positions, interl
     rank = len(qs)
     if not (
         (rank == 4 or rank == 3) and len(ks) == rank and len(cs) == 2 and sin.shape == cs
-        and qs[-1] == ks[-1] and qs[:-2] == ks[:-2] and 0 < 2 * cs[1] <= qs[-1]
+        and qs[-1] == ks[-1] and qs[:-2] == ks[:-2] and 0 < 2 * cs[1] <= qs[-1] < _COUNT_LIMIT
+        and qs[-2] + ks[-2] < _COUNT_LIMIT
         and t in _DTYPES and k.dtype == t and q_weight.dtype == t and k_weight.dtype == t
         and (ct == t or ct == torch.float32) and sin.dtype == ct
         and q_weight.shape == k_weight.shape == (qs[-1],)

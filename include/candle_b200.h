@@ -338,6 +338,8 @@ CB200_API int cb200_qembedding_route_rows(const void* qtable, int qtype, const v
  * Where a call needs scratch memory, `workspace` is device memory of at least the bytes that the
  * matching *_workspace function reports, 16-byte aligned; it is written before it is read, holds
  * nothing between calls, and two calls that may run at the same time need two of them.
+ * Rows have fewer than 2^29 columns and tokens fewer than 2^29 heads, queries and keys together
+ * (CB200_E_UNSUPPORTED_SHAPE).
  */
 
 /*

@@ -311,6 +311,14 @@ class Embedding {
   int64_t hidden_size_;
 };
 
+namespace detail {
+/* A number of columns as the C ABI takes it (which accepts fewer than 2^29). */
+inline int32_t columns(int64_t n) {
+  if (n > INT32_MAX) throw Error("rows of " + std::to_string(n) + " columns, they must be fewer than 2^29");
+  return static_cast<int32_t>(n);
+}
+}  // namespace detail
+
 /* Training and serving operators beside the path (no counterpart in candle; see candle_b200.h for the formulas). */
 namespace ops {
 
@@ -329,14 +337,14 @@ inline void embedding_scaled(const Tensor& table, const Tensor& ids, float scale
   Shape want = ids.dims;
   want.push_back(table.dims[1]);
   detail::check_out(out, want, table.dtype, "embedding");
-  detail::check_rc(cb200_embedding_scaled(table.data, ids.data, out.data, table.dims[0], static_cast<int32_t>(table.dims[1]),
+  detail::check_rc(cb200_embedding_scaled(table.data, ids.data, out.data, table.dims[0], detail::columns(table.dims[1]),
                                           ids.elem_count(), scale, static_cast<int>(table.dtype), detail::id_code(ids.dtype),
                                           status, stream));
 }
 
 inline int64_t embedding_backward_workspace(int64_t vocab, int64_t hidden, int64_t n_ids) {
   int64_t bytes = 0;
-  detail::check_rc(cb200_embedding_backward_workspace(vocab, static_cast<int32_t>(hidden), n_ids, &bytes));
+  detail::check_rc(cb200_embedding_backward_workspace(vocab, detail::columns(hidden), n_ids, &bytes));
   return bytes;
 }
 
@@ -352,14 +360,14 @@ inline void embedding_backward(const Tensor& grad, const Tensor& ids, Tensor& ou
   if (grad.dims != want) throw Error("shape mismatch in embedding-backward " + dims_string(grad.dims) + " " + dims_string(ids.dims));
   detail::check_out(out, {out.dims[0], grad.dims.back()}, out.dtype == DType::F32 ? DType::F32 : grad.dtype, "embedding-backward");
   detail::check_rc(cb200_embedding_backward(grad.data, grad.dims.back(), ids.data, out.data, out.dims[0],
-                                            static_cast<int32_t>(grad.dims.back()), ids.elem_count(), scale, padding_id,
+                                            detail::columns(grad.dims.back()), ids.elem_count(), scale, padding_id,
                                             accumulate ? 1 : 0, static_cast<int>(grad.dtype), static_cast<int>(out.dtype),
                                             detail::id_code(ids.dtype), workspace.data, workspace.bytes, status, stream));
 }
 
 inline int64_t rms_norm_backward_workspace(int64_t rows, int64_t cols) {
   int64_t bytes = 0;
-  detail::check_rc(cb200_rms_norm_backward_workspace(rows, static_cast<int32_t>(cols), &bytes));
+  detail::check_rc(cb200_rms_norm_backward_workspace(rows, detail::columns(cols), &bytes));
   return bytes;
 }
 
@@ -379,7 +387,7 @@ inline void rms_norm_backward(const Tensor& grad, const Tensor& xs, const Tensor
   detail::check_out(dalpha, alpha.dims, DType::F32, "rms-norm-backward");
   const int64_t cols = xs.dims.back(), rows = cols ? xs.elem_count() / cols : 0;
   detail::check_rc(cb200_rms_norm_backward(grad.data, xs.data, alpha.data, grad_sum ? grad_sum->data : nullptr, dxs.data,
-                                           dalpha.data, rows, static_cast<int32_t>(cols), eps, static_cast<int>(xs.dtype),
+                                           dalpha.data, rows, detail::columns(cols), eps, static_cast<int>(xs.dtype),
                                            workspace.data, workspace.bytes, stream));
 }
 
@@ -390,7 +398,7 @@ inline void qk_norm_rope(const cb200_heads& q, const cb200_heads& k, const cb200
 }
 inline int64_t qk_norm_rope_backward_workspace(int64_t dim) {
   int64_t bytes = 0;
-  detail::check_rc(cb200_qk_norm_rope_backward_workspace(static_cast<int32_t>(dim), &bytes));
+  detail::check_rc(cb200_qk_norm_rope_backward_workspace(detail::columns(dim), &bytes));
   return bytes;
 }
 inline void qk_norm_rope_backward(const cb200_heads& grad_q, const cb200_heads& grad_k, const cb200_heads& q, const cb200_heads& k,

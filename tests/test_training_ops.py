@@ -219,6 +219,50 @@ def test_c_entry_points_refuse_on_the_host():
         assert lib.cb200_qk_norm_rope_backward(*args) < 0, i
 
 
+def test_sizes_that_do_not_fit_32_bits_are_refused():
+    import ctypes
+
+    import candle_b200 as cb
+    from candle_b200 import _cabi
+    from candle_b200.ops import _HEADS, _QK_ARGS
+
+    lib, one, unsupported = _cabi.lib, ctypes.c_void_p(16), -5  # never dereferenced
+    n, f32 = ctypes.c_int64(), torch.float32
+    for wide in (1 << 29, (1 << 31) - 1):  # the next power of two would count to a negative number
+        assert lib.cb200_embedding_scaled(one, one, one, 10, wide, 2, 1.0, 0, 1, None, None) == unsupported
+        assert lib.cb200_embedding_backward_workspace(10, wide, 100, ctypes.addressof(n)) == unsupported
+        assert lib.cb200_embedding_backward(one, 8, one, one, 10, wide, 100, 1.0, -1, 0, 0, 0, 1, one, 1 << 60, None, None) == unsupported
+        assert lib.cb200_rms_norm_backward_workspace(4, wide, ctypes.addressof(n)) == unsupported
+        assert lib.cb200_rms_norm_backward(one, one, one, None, one, one, 4, wide, 1e-5, 0, one, 1 << 60, None) == unsupported
+        assert lib.cb200_qk_norm_rope_backward_workspace(wide, ctypes.addressof(n)) == unsupported
+        for dim, heads in ((wide, 1), (2, wide)):
+            h = _HEADS.pack(16, 2 * wide, 2 * wide, dim, heads, 0)
+            args = _QK_ARGS.pack(16, 16, 16, 16, 16, 1, 1, 7, dim, 2, 1e-5, 0, 0, 0, 2, 0)
+            assert lib.cb200_qk_norm_rope(h, h, h, h, args, None, None) == unsupported
+            assert lib.cb200_qk_norm_rope_backward(h, h, h, h, h, h, one, one, args, one, 1 << 60, None, None) == unsupported
+    half = _HEADS.pack(16, 1 << 32, 1 << 32, 2, 1 << 30, 0)  # whose sum would be negative
+    args = _QK_ARGS.pack(16, 16, 16, 16, 16, 1, 1, 7, 2, 2, 1e-5, 0, 0, 0, 2, 0)
+    assert lib.cb200_qk_norm_rope(half, half, half, half, args, None, None) == unsupported
+
+    def meta(*shape, dtype=f32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    ids = meta(2, dtype=torch.int64)
+    for wide in (1 << 29, (1 << 32) + 8):  # the second is 8 in 32 bits
+        with pytest.raises(cb.CandleError, match=str(wide)):
+            cb.embedding_scaled(meta(3, wide), ids, 2.0)
+        with pytest.raises(cb.CandleError, match=str(wide)):
+            cb.embedding_backward(meta(2, wide), ids, 10)
+        with pytest.raises(cb.CandleError, match=str(wide)):
+            cb.rms_norm_backward(meta(2, wide), meta(2, wide), meta(wide), 1e-5)
+        for dim, heads in ((wide, 1), (2, wide)):
+            q, k, w, c = meta(1, heads, dim), meta(1, 1, dim), meta(dim), meta(1, 1)
+            with pytest.raises(cb.CandleError, match=str(wide)):
+                cb.qk_norm_rope(q, k, w, w, 1e-5, c, c)
+            with pytest.raises(cb.CandleError, match=str(wide)):
+                cb.qk_norm_rope_backward(q, k, q, k, w, w, 1e-5, c, c)
+
+
 def test_a_padding_id_is_a_row_of_the_table():
     import ctypes
 
