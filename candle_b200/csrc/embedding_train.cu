@@ -444,6 +444,9 @@ struct SumArgs {
 };
 constexpr int kChunkBatch = 8;
 constexpr int kTokenBatch = 8;
+// Up to so many tokens a CTA adds even the longest run while the others are added (at most 16 batches of loads per warp);
+// beyond, the launch for the chunks pays (3001 skewed tokens of 1000 columns: 58 us without, 41 with it).
+constexpr int kDirectMax = 1024;
 
 template <int DT, int VEC>
 __device__ __forceinline__ void add_unit(const Unit<DT, VEC>& u, float (&acc)[VEC]) {
@@ -960,13 +963,13 @@ Workspace lay_out(void* base, int64_t vocab, int hidden, int64_t n) {
   for (int i = 0; i < 2; ++i) {
     w.keys[i] = reinterpret_cast<uint32_t*>(take(n * 4));
     w.values[i] = reinterpret_cast<uint32_t*>(take(n * 4));
-    w.counts[i] = reinterpret_cast<uint32_t*>(take(int64_t(kSortMaxCtas) * kSortMaxBins * 4));
+    w.counts[i] = reinterpret_cast<uint32_t*>(take(n > kRankMax ? int64_t(kSortMaxCtas) * kSortMaxBins * 4 : 0));
   }
   w.counters = reinterpret_cast<Counters*>(take(sizeof(Counters)));
   w.long_runs = reinterpret_cast<uint2*>(take(n / kLongRun * 8));
   w.begins = reinterpret_cast<uint32_t*>(take(vocab * 4));
   w.present = take(vocab);
-  w.chunk_sums = reinterpret_cast<float*>(take(n / kChunk * hidden * 4));
+  w.chunk_sums = reinterpret_cast<float*>(take(n > kDirectMax ? n / kChunk * hidden * 4 : 0));
   w.bytes = at;
   return w;
 }
@@ -1053,9 +1056,7 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
   s.units = a.hidden / VEC;
   s.tiles = (s.units + 31) / 32;
   const int64_t sms = sm_count();
-  // Up to 1024 tokens a CTA adds even the longest run while the others are added (at most 16 batches of loads per warp);
-  // beyond, the launch for the chunks pays (3001 skewed tokens of 1000 columns: 58 us without, 41 with it).
-  const bool chunks = a.n_ids > 1024;
+  const bool chunks = a.n_ids > kDirectMax;
   const bool few = a.n_ids <= kRankMax;  // short kernels one behind the other: their launches overlap
   if (chunks) {
     s.chunk_sums = w.chunk_sums;

@@ -472,6 +472,8 @@ bool launch_fast(const RmsBackwardArgs& a, float* partials, cudaStream_t stream,
   return true;
 }
 
+constexpr int kMaxElements = 32;  // per thread
+
 template <int DT, int E>
 cudaError_t launch_elements(const FastArgs& f, cudaStream_t stream) {
   const size_t input = 2 * static_cast<size_t>(visit_bytes(kThreads >> f.tpr_shift, f.a.n, Elem<DT>::kBytes));
@@ -506,8 +508,8 @@ cudaError_t launch_dt(const RmsBackwardArgs& a, float* partials, float2* factors
   if constexpr (DT != kDtF32)
     if (at % 4 == 0 && launch_fast<DT, 4>(a, partials, stream, &e)) return e;
   FastArgs f{a, partials, 3, a.n};
-  const int elements = split_row(f, 32, kThreads);
-  if (elements > 32) return launch_long<DT>(a, partials, factors, stream);
+  const int elements = split_row(f, kMaxElements, kThreads);
+  if (elements > kMaxElements) return launch_long<DT>(a, partials, factors, stream);
   if (elements <= 8) return launch_elements<DT, 8>(f, stream);
   if (elements <= 16) return launch_elements<DT, 16>(f, stream);
   return elements <= 24 ? launch_elements<DT, 24>(f, stream) : launch_elements<DT, 32>(f, stream);
@@ -521,16 +523,21 @@ cudaError_t launch_sum_partials(const float* partials, int n_partials, int cols,
                           cols, out, split, out2);
 }
 
+// Bytes of the lines of partial sums: no grid has more CTAs, or slices, than there are rows.
+static int64_t partial_bytes(int64_t rows, int n) {
+  const int64_t lines = rows < max_partials() ? rows : max_partials();
+  return (lines * n * 4 + 15) & ~int64_t(15);
+}
+
+// Behind them the factors of the rows, for lengths that may take the three passes.
 int64_t rms_backward_workspace(int64_t rows, int n) {
-  const int64_t partials = (static_cast<int64_t>(max_partials()) * n * 4 + 15) & ~int64_t(15);
-  return partials + rows * 8;
+  return partial_bytes(rows, n) + (n > kThreads * kMaxElements ? rows * 8 : 0);
 }
 
 cudaError_t launch_rms_backward(int dtype, const RmsBackwardArgs& a, void* workspace, cudaStream_t stream) {
   if (a.rows == 0) return cudaMemsetAsync(a.dalpha, 0, static_cast<size_t>(a.n) * 4, stream);
   float* partials = static_cast<float*>(workspace);
-  float2* factors = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
-                                              ((static_cast<int64_t>(max_partials()) * a.n * 4 + 15) & ~int64_t(15)));
+  float2* factors = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + partial_bytes(a.rows, a.n));
   switch (dtype) {
     case kDtF32: return launch_dt<kDtF32>(a, partials, factors, stream);
     case kDtF16: return launch_dt<kDtF16>(a, partials, factors, stream);

@@ -263,6 +263,30 @@ def test_sizes_that_do_not_fit_32_bits_are_refused():
                 cb.qk_norm_rope_backward(q, k, q, k, w, w, 1e-5, c, c)
 
 
+def test_workspaces_grow_with_the_call():
+    import ctypes
+
+    from candle_b200 import _cabi
+
+    n = ctypes.c_int64()
+
+    def size(name, *args):
+        assert getattr(_cabi.lib, name)(*args, ctypes.addressof(n)) == 0
+        return n.value
+
+    # a line of f32 partial sums per row at most, and 8 bytes per row that is too long for one pass
+    for rows, cols in ((1, 8), (1, 16384), (1, 1 << 20), (3, 8192), (7, 8193), (2, (1 << 29) - 1)):
+        assert rows * cols * 4 <= size("cb200_rms_norm_backward_workspace", rows, cols) <= rows * (cols * 4 + 8) + 16, (rows, cols)
+    many = size("cb200_rms_norm_backward_workspace", 1 << 20, 256)
+    assert many == size("cb200_rms_norm_backward_workspace", 1 << 21, 256)  # no more lines than the GPU runs CTAs
+    assert size("cb200_rms_norm_backward_workspace", 1 << 20, 8193) - size("cb200_rms_norm_backward_workspace", 1 << 20, 8192) >= 8 << 20
+    # sorted ids and positions twice, five bytes per row of the table, the long runs; an f32 row per 32 ids above 1024 ids
+    for vocab, hidden, ids in ((10, 8, 1), (1000, 8192, 1024), (10, 1 << 20, 64), (100, 64, 8192)):
+        sums = ids // 32 * hidden * 4 if ids > 1024 else 0
+        least = 16 * ids + 5 * vocab + sums
+        assert least <= size("cb200_embedding_backward_workspace", vocab, hidden, ids) <= least + ids // 8 + 10 * 16, (vocab, hidden, ids)
+
+
 def test_a_padding_id_is_a_row_of_the_table():
     import ctypes
 
@@ -566,6 +590,47 @@ def test_rms_norm_backward_odd_rows_and_refusals(cb):
     buf = torch.zeros(5, 512, device="cuda")
     with pytest.raises(cb.CandleError, match="overlaps"):
         cb.rms_norm_backward(buf[:4], buf[:4].clone(), torch.ones(512, device="cuda"), 1e-5, out=buf[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(2, 1 << 20), (1, 300001), (300, 9000)])
+def test_rms_norm_backward_of_very_long_rows(cb, rows, cols):
+    x, grad, w = rand(1, (rows, cols), torch.float32), rand(2, (rows, cols), torch.float32), rand(3, (cols,), torch.float32, 1.0, 0.1)
+    dx, size, dw, dw_size = norm_grad_64(grad, x, w, 1e-5)
+    got, got_w = cb.rms_norm_backward(grad, x, w, 1e-5)
+    check(got, dx, (2 * SUM(cols) + OPS) * U * size)
+    check(got_w, dw, (rows + SUM(cols) + OPS) * U * dw_size)
+
+
+@pytest.mark.gpu
+def test_nothing_behind_the_workspace_is_written(cb):
+    import ctypes
+
+    from candle_b200 import _cabi
+
+    tail, stream, n = 1 << 20, torch.cuda.current_stream().cuda_stream, ctypes.c_int64()
+
+    def workspace(name, *args):
+        assert getattr(_cabi.lib, name)(*args, ctypes.addressof(n)) == 0
+        assert n.value % 16 == 0
+        return torch.full((n.value + tail,), 0xA5, dtype=torch.uint8, device="cuda"), n.value
+
+    # the smallest calls, both sides of the sizes where scratch changes, and lengths for every route
+    for rows, cols in ((1, 8), (1, 9), (5, 64), (600, 8192), (2, 8191), (3, 8193), (700, 8193), (1, 50000), (3000, 264)):
+        x, grad, w = rand(1, (rows, cols), torch.float32), rand(2, (rows, cols), torch.float32), rand(3, (cols,), torch.float32)
+        ws, size = workspace("cb200_rms_norm_backward_workspace", rows, cols)
+        dx, dw = torch.empty_like(x), torch.empty(cols, device="cuda")
+        _cabi.call("cb200_rms_norm_backward", grad.data_ptr(), x.data_ptr(), w.data_ptr(), None, dx.data_ptr(), dw.data_ptr(), rows, cols,
+                   1e-5, 0, ws.data_ptr(), size, stream)
+        want, want_w = cb.rms_norm_backward(grad, x, w, 1e-5)
+        assert torch.equal(dx, want) and torch.equal(dw, want_w) and (ws[size:] == 0xA5).all(), (rows, cols)
+    for ids, vocab, hidden in ((1, 1, 8), (64, 3, 65), (1024, 5, 24), (1025, 5, 24), (8192, 70, 8), (8193, 70, 8), (40000, 1 << 19, 8)):
+        grad, which = rand(4, (ids, hidden), torch.float32), make_ids(5, ids, vocab, "skew")
+        ws, size = workspace("cb200_embedding_backward_workspace", vocab, hidden, ids)
+        out = torch.empty(vocab, hidden, device="cuda")
+        _cabi.call("cb200_embedding_backward", grad.data_ptr(), hidden, which.data_ptr(), out.data_ptr(), vocab, hidden, ids, 1.0, -1, 0, 0, 0, 2,
+                   ws.data_ptr(), size, None, stream)
+        assert torch.equal(out, cb.embedding_backward(grad, which, vocab)) and (ws[size:] == 0xA5).all(), (ids, vocab, hidden)
 
 
 # ---- head norms with rotation ------------------------------------------------------------------------------
