@@ -1035,3 +1035,70 @@ def test_sort_digits_cover_every_key():
         width = -(-bits // passes)
         assert width <= 9 and passes * width >= bits and (passes - 1) * width < 32
         assert np.uint32(vocab) >> np.uint32((passes - 1) * width) < (1 << width)
+
+
+@pytest.mark.gpu
+def test_operators_in_two_host_threads(cb):
+    """Two threads on streams of their own run the step with different shapes, the first calls of the process's cached sizes
+    among them."""
+    import threading
+
+    sets = [block_inputs(torch.bfloat16, 600 + 50 * i, b=2 + 3 * i, t=41 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(100):
+                    got[k] = [*got[k][-3:], block_step(cb, *sets[k])]
+        except Exception as e:  # noqa: BLE001  (reported by the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for k, s in enumerate(sets):
+        want = block_step(cb, *s)
+        for outs in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), k
+
+
+@pytest.mark.gpu
+def test_cpp_mirror_computes_what_the_package_does(cb, tmp_path):
+    import os
+    import shutil
+    import subprocess
+
+    gxx, cuda = shutil.which("g++"), "/usr/local/cuda"
+    if gxx is None or not os.path.exists(os.path.join(cuda, "include", "cuda_runtime.h")):
+        pytest.skip("no g++ or no CUDA runtime headers")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib_dir, exe = os.path.join(root, "candle_b200", "_lib"), str(tmp_path / "training_gpu")
+    subprocess.run([gxx, "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(root, "include"), "-isystem", os.path.join(cuda, "include"),
+                    "-o", exe, os.path.join(root, "tests", "cpp", "training_gpu.cpp"), "-L", lib_dir, "-l:libcandle_b200.so",
+                    f"-Wl,-rpath,{lib_dir}", "-L", os.path.join(cuda, "lib64"), "-lcudart"], check=True)
+    vocab, hidden, n, hq, hk, d, f32 = 40, 136, 90, 4, 2, 48, torch.float32
+    t = {name: rand(50 + i, shape, f32) for i, (name, shape) in enumerate({
+        "table": (vocab, hidden), "alpha": (hidden,), "grad": (2, n // 2, hidden), "extra": (2, n // 2, hidden), "sum": (vocab, hidden),
+        "q": (n, hq, d), "k": (n, hk, d), "gq": (n, hq, d), "gk": (n, hk, d), "wq": (d,), "wk": (d,), "cos": (n, d // 2), "sin": (n, d // 2)}.items())}
+    ids = make_ids(49, n, vocab, "skew").view(2, n // 2)
+    for name, x in (*t.items(), ("ids", ids.to(torch.int32))):
+        x.cpu().numpy().tofile(tmp_path / name)
+    out = subprocess.run([exe, str(tmp_path), *map(str, (vocab, hidden, n, hq, hk, d))], capture_output=True, text=True)
+    assert out.returncode == 0, (out.returncode, out.stdout + out.stderr)
+    y = cb.embedding_scaled(t["table"], ids, 3.0)
+    dx, dalpha = cb.rms_norm_backward(t["grad"], y, t["alpha"], 1e-5, grad_sum=t["extra"])
+    heads = (t["q"], t["k"], t["wq"], t["wk"], 1e-5, t["cos"], t["sin"])
+    oq, ok = cb.qk_norm_rope(*heads, interleaved=True)
+    dq, dk, dwq, dwk = cb.qk_norm_rope_backward(t["gq"], t["gk"], *heads, interleaved=True)
+    want = dict(y=y, dtable=cb.embedding_backward(t["grad"], ids, vocab, scale=3.0),
+                sum=cb.embedding_backward(t["grad"], ids, vocab, scale=3.0, out=t["sum"].clone(), accumulate=True, padding_id=1),
+                dx=dx, dalpha=dalpha, oq=oq, ok=ok, dq=dq, dk=dk, dwq=dwq, dwk=dwk)
+    for name, w in want.items():
+        got = torch.from_numpy(np.fromfile(tmp_path / f"out.{name}", np.float32)).view(w.shape)
+        assert torch.equal(got, w.cpu()), name
