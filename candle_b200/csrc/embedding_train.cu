@@ -82,10 +82,14 @@ __device__ __forceinline__ void store_floats(void* base, int64_t elem, const flo
 }
 
 // ---------------------------------------------------------------------------------------------
-// Scaled lookup: a warp per (token, tile of 32 U units), its loads in flight together
+// Scaled lookup: a warp per (token, tile of 32 U units), its loads in flight together.  Four units per lane whatever the
+// number of rows: with one, which spreads few rows over more warps, 1 to 16 rows take the same time within 0.1 us, 592 rows of
+// 4096 bf16 columns 3.7 us on the device instead of 3.3, 8192 rows 20.7 instead of 18.0.
 // ---------------------------------------------------------------------------------------------
-template <int DT, int VEC, int U>
+constexpr int kLookupUnits = 4;
+template <int DT, int VEC>
 __global__ void __launch_bounds__(256) scaled_lookup_kernel(const ScaledLookupArgs a, int units, int tiles) {
+  constexpr int U = kLookupUnits;
   const int lane = threadIdx.x & 31;
   const int64_t n_warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
   const int64_t n_items = a.n_ids * tiles;
@@ -112,23 +116,21 @@ __global__ void __launch_bounds__(256) scaled_lookup_kernel(const ScaledLookupAr
   }
 }
 
-template <int DT, int VEC, int U>
+template <int DT, int VEC>
 cudaError_t launch_scaled_lookup_t(const ScaledLookupArgs& a, cudaStream_t stream) {
-  const int units = a.hidden / VEC, tiles = (units + 32 * U - 1) / (32 * U);
+  const int units = a.hidden / VEC, tiles = (units + 32 * kLookupUnits - 1) / (32 * kLookupUnits);
   int64_t grid = (a.n_ids * tiles + 7) / 8;
   const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
   if (grid > cap) grid = cap;
-  scaled_lookup_kernel<DT, VEC, U><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, units, tiles);
+  scaled_lookup_kernel<DT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, units, tiles);
   return cudaGetLastError();
 }
 
 template <int DT>
 cudaError_t launch_scaled_lookup_dt(const ScaledLookupArgs& a, cudaStream_t stream) {
   constexpr int kPV = Elem<DT>::kPerVec;
-  if (a.hidden % kPV != 0 || !aligned_to(a.table, 16) || !aligned_to(a.out, 16)) return launch_scaled_lookup_t<DT, 1, 4>(a, stream);
-  // few rows: one vector per lane spreads them over more warps
-  if (a.n_ids * (a.hidden / kPV) < static_cast<int64_t>(sm_count()) * 2048) return launch_scaled_lookup_t<DT, kPV, 1>(a, stream);
-  return launch_scaled_lookup_t<DT, kPV, 4>(a, stream);
+  if (a.hidden % kPV != 0 || !aligned_to(a.table, 16) || !aligned_to(a.out, 16)) return launch_scaled_lookup_t<DT, 1>(a, stream);
+  return launch_scaled_lookup_t<DT, kPV>(a, stream);
 }
 
 // The caller's ids.
