@@ -2,19 +2,21 @@
 //
 // Gradient: out[v] = scale * sum of grad[i] over the tokens i with ids[i] == v.  The tokens are sorted by id
 // (stable, as (id, position) pairs), so each table row owns a contiguous run of the sorted list and its sum has a
-// fixed order: no floating-point atomics, equal inputs give equal bits.  Then
+// fixed order: no floating-point atomics, and equal inputs of equal alignment and strides give equal bits (alignment decides
+// the width of the tiles, and the number of tiles whether a warp or a CTA adds a long run of up to 511 tokens).  Then
 //   - chunk_sums_kernel adds up every aligned chunk of 32 sorted tokens that belongs to one id: text is skewed
 //     (the hottest id of 65536 tokens has thousands) and this is what spreads a long run over the GPU;
-//   - row_stream_kernel adds the runs.  A CTA per SM begins with the long ones (64 tokens and more: their chunk sums and the
-//     ends that do not fill a chunk), whose chains of dependent loads the other CTAs' traffic hides.  For the others
+//   - row_stream_kernel adds the runs.  A CTA per SM begins with the long ones (64 tokens and more: the ends that do not
+//     fill a chunk, then their chunk sums), whose chains of dependent loads the other CTAs' traffic hides.  For the others
 //     work is cut by tokens, not by rows, since a few rows of a text's table have most of its tokens: a warp takes the
 //     runs that begin at a few neighbouring sorted positions.
 // The rows without tokens are filled with zeros by further blocks of the launches that leave the memory idle: the radix
 // sort's, or with few tokens the chunk sums' or the row sums'.
 //
-// Measured (B200): 65536 Zipf-distributed tokens, 128256 x 4096 bf16 (537 MB of gradients in, 1051 MB out): 298 us, 5.3 TB/s
+// Measured (B200): 65536 Zipf-distributed tokens, 128256 x 4096 bf16 (537 MB of gradients in, 1051 MB out): 295 us, 5.4 TB/s
 // (the long runs in a launch of their own: 312); 4096 tokens added to a 32000 x 4096 f32 table (160 MB): 43 us; 46 tokens,
-// 81761 x 2504 f32 (819 MB of zeros): 119 us.  Below some 8000 tokens the time is the latency of the three to four launches.
+// 81761 x 2504 f32 (819 MB of zeros): 114 us.  Rows that are not whole, aligned 16-byte vectors go by elements: 16384 skewed tokens, 30000 x 4097
+// bf16 182 us (4096 columns: 93), the lookup of 16384 such rows 67 us (44), of 2731 f32 columns 60 us.  Below some 8000 tokens the time is the latency of the three to four launches.
 #include "launch.h"
 
 namespace cb200 {
@@ -218,7 +220,7 @@ constexpr int kSortThreads = 512;
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kRankThreads = 256;
 constexpr int kRankWarps = kRankThreads / 32;
-constexpr int kRankMax = 8192;
+constexpr int kRankMax = 8192;  // 2000 rows of 512 bf16 columns: 1024 skewed tokens 20.1 us (radix 27.6), 6000 39.8 (41.4), 8192 44.6 (43.3)
 constexpr int kSortMaxBits = 9;
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 constexpr int kSortMaxCtas = 512;
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kRankThreads) sort_small_kernel(const SortArgs
 // Sums over the sorted tokens
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunk = 32;            // sorted tokens per chunk sum
-constexpr int kLongRun = 2 * kChunk;  // runs of at least this many tokens contain a whole chunk and are added by a CTA
+constexpr int kLongRun = 2 * kChunk;  // runs of at least this many tokens contain a whole chunk and are added apart from the others
 constexpr int kMaxGroup = 16;         // sorted positions per warp and visit, at most: with kLongRun - 1 behind them fewer than 96
 
 struct SumArgs {
@@ -446,8 +448,9 @@ struct SumArgs {
 };
 constexpr int kChunkBatch = 8;
 constexpr int kTokenBatch = 8;
-// Up to so many tokens a CTA adds even the longest run while the others are added (at most 16 batches of loads per warp);
-// beyond, the launch for the chunks pays (3001 skewed tokens of 1000 columns: 58 us without, 41 with it).
+// Up to so many tokens a CTA adds even the longest run, token by token (at most 128 additions per warp, then the eight warps).
+// The launch for the chunks keeps the additions in a row few and the longest run short; 4096 skewed tokens of 1000 columns
+// over 2000 rows take 36.9 us with it and 38.4 without, 3001 32.6 and 31.9, 1024 25.4 and 21.3, 256 21.1 and 17.6.
 constexpr int kDirectMax = 1024;
 
 template <int DT, int VEC>
@@ -616,7 +619,10 @@ __device__ __forceinline__ void finish_run(const SumArgs& a, uint32_t key, int u
 // With chunk sums and many of them: eight (run, tile) items per CTA at a time, a warp for each run of fewer
 // than kWarpRun tokens; the others take a CTA each, every warp every eighth piece, then the warps' sums in order.  The eight
 // lie far apart in the list, so that the tiles of a hot run go to different CTAs (65536 tokens over 1000 rows of
-// 8192: 343 us with neighbours, 284 so).
+// 8192: 343 us with neighbours, 284 so).  "Many" is beyond 12 items per CTA: below, one warp's chain of loads is what is
+// waited for (2000 tokens over 10 rows of 64 columns: 27.8 us by warps, 18.5 by CTAs), above, the CTAs' barriers (40000 over
+// 300 rows of 4096: 129 by warps, 160 by CTAs).  kWarpRun: 65536 tokens over 200 rows of 4096 151 us with 512, 175 with 256;
+// no difference in text's skew.
 constexpr int kWarpRun = 512;
 template <int VEC>
 constexpr size_t kLongShared = size_t(8) * 32 * VEC * 4 + size_t(8) * kPieces * PieceRing<VEC>::kWords * 32 * 16;
@@ -1080,7 +1086,9 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     s.group = kMaxGroup;
     while (s.group > 1 && (a.n_ids + s.group - 1) / s.group * tiles < sms * per_sm * 8 * 4) s.group /= 2;
     const int64_t items = (a.n_ids + s.group - 1) / s.group * tiles;
-    // a CTA per SM begins with the long runs, if there are any (two: 305 instead of 298 us for 65536 skewed tokens)
+    // A CTA per SM begins with the long runs, if there are any.  With two, text's skew loses (65536 tokens of 4096 columns over
+    // 128256 rows 285 -> 287 us in a graph, 16384 over 32000 97 -> 99), many tokens per row gain (65536 of 8192 columns over 1000 rows,
+    // uniform: 349 -> 309).
     const int64_t long_items = a.n_ids < kLongRun ? 0 : (chunks ? a.n_ids / kLongRun : (a.n_ids + kLongRun - 1) / kLongRun) * s.tiles;
     s.long_blocks = static_cast<unsigned>(long_items < sms ? long_items : sms);
     s.share = few ? 0 : 1;
@@ -1089,9 +1097,10 @@ cudaError_t launch_sums(const TableGradArgs& a, const Workspace& w, int where, Z
     return launch_dependent(few, kern, s.long_blocks + static_cast<unsigned>(blocks) + s.zero.blocks, 256, smem, stream, s);
   };
   if constexpr (VEC > 1) {
-    // Two vectors per lane share what a token costs in instructions (65536 skewed tokens of 4096 columns: 341 us with one,
-    // 297 with two); one keeps more warps busy where there are not four such items for each.  Four make the items so
-    // large that the last ones are waited for: 115 us instead of 104 for 16384 tokens.
+    // Two vectors per lane share what a token costs in instructions (65536 skewed tokens of 4096 columns over 128256 rows: 302 us
+    // with one, 283 with two; 16384 uniform ones over 2000 rows 72 and 66); one keeps more warps busy where there are not four
+    // such items for each (1024 skewed tokens over 2000 rows: 26.1 and 29.2; 1776, about the limit, 35.8 and 37.7, but uniform
+    // 26.5 and 24.8).  Four make the items so large that the last ones are waited for: 115 us instead of 104 for 16384 tokens.
     constexpr size_t kSmem = size_t(8) * (ACC ? 8 : 16) * 32 * (16 + (ACC ? VEC * Elem<DTO>::kBytes : 0));
     if (s.units > 32 && a.n_ids * ((s.units + 63) / 64) >= sms * 24 * 4) return finish(row_stream_kernel<DT, DTO, ACC, 2>, 2, kSmem);
     return finish(row_stream_kernel<DT, DTO, ACC, 1>, 1, kSmem);

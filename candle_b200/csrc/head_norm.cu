@@ -730,6 +730,10 @@ cudaError_t launch_forward_pv(const ForwardArgs& a, cudaStream_t stream, bool* d
     const Walk w = plan_walk(c, c.q_heads, c.k_heads, items, 1, cap, grid);
     return launch_forward_vec<DT, DTC, PV, 2, 1>(a, w, grid, stream);
   }
+  // Few units: a row per lane and unit, so that more warps have one.  Device times so and with kRows: 32 + 8 bf16 heads of 128 (the
+  // limit is 1421 tokens) 64 tokens 2.3 and 2.7 us, 256 3.1 both, 1024 6.7 and 5.9, 2048 10.9 and 8.8; 16 + 2 f32 heads of 64
+  // (2368 tokens) 256 2.7 and 2.8, 900 4.0 and 3.5, 1300 4.5 and 4.8, 2000 6.1 and 5.5.  In the last factor of two below the limit
+  // it depends on how the units fill the warps.
   constexpr int kRows = kUnitRows<DT, PV>;
   Walk w = plan_walk(c, c.q_heads, c.k_heads, items, kRows, cap, grid);
   if (w.n_units >= 2 * cap * kWarps) return launch_forward_vec<DT, DTC, PV, 1, kRows>(a, w, grid, stream);

@@ -21,7 +21,7 @@ void set_wait_tuning(WaitTuning t);
 // Launches a kernel that begins with follow_previous() behind the kernel launched last on `stream`, which is one of the
 // same call and does so too: with `overlap` its launch overlaps that kernel's end, which saves about 1.5 us.  Not behind a
 // kernel that keeps the memory busy with loads into registers for long: shared memory of the waiting CTAs takes L1 from
-// them (the sums of 65536 tokens of 8192 columns: 370 us without, 512 with).
+// them (table gradient of 65536 tokens over 1000 rows of 8192 columns: 350 us without, 377 with).
 template <typename... P, typename... A>
 cudaError_t launch_dependent(bool overlap, void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
                              const A&... args) {

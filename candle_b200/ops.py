@@ -436,8 +436,8 @@ def qembedding_route_rows(qtensor, ids: torch.Tensor, dst_ptrs, row_bounds, *, v
 
 
 # ---- training and serving operators beside the path -------------------------------------------------
-# f32 inside with one rounding to the output's type; the sums of gradients are held in f32 and have a fixed
-# order, so equal inputs give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
+# f32 inside with one rounding to the output's type; the sums of gradients are held in f32 and have an order that
+# shapes, ids, alignment and strides fix, so equal inputs laid out alike give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
 
 
 _COUNT_LIMIT = 1 << 29  # columns of a row, heads of a token: the kernels count them in 32 bits
@@ -564,7 +564,8 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
                        padding_id: int | None = None, check: bool = True,
                        status: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of ``scale * Embedding::forward(ids)`` with respect to the ``[vocab, hidden]`` table: row v is
-    ``scale`` times the sum of the rows of ``grad`` whose id is v, in f32 and in the order of the tokens.
+    ``scale`` times the sum of the rows of ``grad`` whose id is v, in f32 and in a fixed order (that of the tokens up to
+    63 of them; longer runs are added in parts).
 
     ``grad`` is ``[*ids.shape, hidden]`` (rows may be strided).  The result is a fresh tensor of ``out_dtype``
     (``grad``'s, or f32) or ``out``; every row is written, zeros where no id points.  With ``accumulate`` the sums are

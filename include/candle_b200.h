@@ -334,7 +334,8 @@ CB200_API int cb200_qembedding_route_rows(const void* qtable, int qtype, const v
  * ---- Training and serving operators beside the path above (no counterpart in the reference, whose
  * fused ops have no backward: CustomOp2/3 with `apply_op*_no_bwd`, candle-nn/src/ops.rs:651, 908).
  * Their arithmetic is f32 inside with ONE rounding to the output's type; sums of gradients are held in
- * f32 and taken in an order that depends on the shapes and the ids alone, so equal inputs give equal bits on one kind of GPU.
+ * f32 and taken in an order that depends on the shapes, the ids, and the alignment and strides of the tensors alone (these
+ * choose the kernel), so equal inputs laid out alike give equal bits on one kind of GPU.
  * Where a call needs scratch memory, `workspace` is device memory of at least the bytes that the
  * matching *_workspace function reports, 16-byte aligned; it is written before it is read, holds
  * nothing between calls, and two calls that may run at the same time need two of them.
