@@ -437,7 +437,8 @@ def qembedding_route_rows(qtensor, ids: torch.Tensor, dst_ptrs, row_bounds, *, v
 
 # ---- training and serving operators beside the path -------------------------------------------------
 # f32 inside with one rounding to the output's type; the sums of gradients are held in f32 and have an order that
-# shapes, ids, alignment and strides fix, so equal inputs laid out alike give equal bits.  Scratch memory comes from torch's allocator, one piece per call.
+# shapes, ids, alignment and strides fix, so equal inputs laid out alike give equal bits.  Scratch memory comes from
+# torch's allocator, one piece per call.
 
 
 _COUNT_LIMIT = 1 << 29  # columns of a row, heads of a token: the kernels count them in 32 bits
